@@ -1,0 +1,243 @@
+"""Gated linear recurrence h_t = a_t h_{t-1} + u_t over sequences, its backward pass and its single-token step
+(csrc/scan.hip).  It stands beside the n-step return assembly (agents/nstep.py, which walks one episode step by step on the
+host): discounted returns are this recurrence with gate = gamma, run backwards, and so is a recurrent layer's memory.
+The evaluator's return report (agent_params.evaluate_returns) runs on it.
+
+On CPU tensors the same functions compute the same formulas in torch, step by step.
+"""
+import ctypes
+
+import torch
+
+from ._seq import TYPE_CODES, check_floating, check_int, launched, native, on_device, ptr, stream_of
+
+GATES = ("decay", "logit")
+_vp, _i64, _int = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
+
+
+class _Args(ctypes.Structure):      # mirrors ScanArgs in csrc/scan.hip
+    _fields_ = [("x", _vp), ("gate", _vp), ("dh", _vp), ("xs", _i64 * 3), ("gs", _i64 * 3), ("ds", _i64 * 3), ("h0", _vp),
+                ("dlast", _vp), ("lengths", _vp), ("len64", _int), ("h", _vp), ("last", _vp), ("hist", _vp), ("dx", _vp),
+                ("dg", _vp), ("dh0", _vp), ("B", _int), ("T", _int), ("D", _int), ("logit", _int), ("mix", _int),
+                ("reverse", _int)]
+
+
+class _StepArgs(ctypes.Structure):  # mirrors ScanStepArgs
+    _fields_ = [("x", _vp), ("gate", _vp), ("state", _vp), ("state_out", _vp), ("h", _vp), ("xs", _i64 * 2),
+                ("gs", _i64 * 2), ("ss", _i64 * 2), ("os", _i64 * 2), ("B", _int), ("D", _int), ("logit", _int),
+                ("mix", _int)]
+
+
+def _gate(g, logit):
+    """-> (a, 1 - a) in 32 bits"""
+    g = g.float()
+    return (torch.sigmoid(g), torch.sigmoid(-g)) if logit else (g, 1 - g)
+
+
+def _advance(h, x, g, logit, mix):
+    a, c = _gate(g, logit)
+    x = x.float()
+    return _decayed(h, a, c, logit) + (c * x if mix else x)
+
+
+def _decayed(h, a, c, logit):
+    """a h (csrc/scan.hip: from 1 - a where a gate is above 1/2)"""
+    return torch.where(c <= 0.5, h - c * h, a * h) if logit else a * h
+
+
+def _steps(T, n, reverse, dev):
+    """Yields, for every step of the recurrence, the position it reads per sequence and whether that step exists."""
+    for i in range(T):
+        pos = (n - 1 - i).clamp_min(0) if reverse else torch.full_like(n, i)
+        yield pos, (i < n)[:, None]
+
+
+def _forward_torch(x, gate, h0, n, logit, mix, reverse):
+    B, T, D = x.shape
+    row = torch.arange(B)
+    h = h0.clone() if h0 is not None else torch.zeros(B, D)
+    out, hist = torch.zeros(B, T, D, dtype=x.dtype), []
+    for pos, on in _steps(T, n, reverse, x.device):
+        hist.append(h)
+        h = torch.where(on, _advance(h, x[row, pos], gate[row, pos], logit, mix), h)
+        out[row, pos] = torch.where(on, h.to(x.dtype), out[row, pos])
+    return out, h, hist
+
+
+def _backward_torch(x, gate, h0, n, logit, mix, reverse, dh, dlast):
+    B, T, D = x.shape
+    row = torch.arange(B)
+    hist = _forward_torch(x, gate, h0, n, logit, mix, reverse)[2]
+    dx, dg = torch.zeros(B, T, D, dtype=x.dtype), torch.zeros(B, T, D, dtype=x.dtype)
+    carry = dlast.clone() if dlast is not None else torch.zeros(B, D)
+    for prev, (pos, on) in reversed(list(zip(hist, _steps(T, n, reverse, x.device)))):
+        a, c = _gate(gate[row, pos], logit)
+        xv = x[row, pos].float()
+        gr = carry + (dh[row, pos].float() if dh is not None else 0.0)
+        da = gr * (prev - xv if mix else prev)
+        if logit:
+            da = da * a * c
+        dx[row, pos] = torch.where(on, (gr * c if mix else gr).to(x.dtype), dx[row, pos])
+        dg[row, pos] = torch.where(on, da.to(x.dtype), dg[row, pos])
+        carry = torch.where(on, _decayed(gr, a, c, logit), carry)
+    return dx, dg, carry
+
+
+def _lengths(lengths, B, T):
+    return torch.full((B,), T) if lengths is None else lengths.long().clamp(0, T)
+
+
+def _fill(args, x, gate, h0, lengths, how):
+    args.x, args.gate, args.h0, args.lengths = ptr(x), ptr(gate), ptr(h0), ptr(lengths)
+    args.xs[:], args.gs[:] = x.stride(), gate.stride()
+    args.len64 = int(lengths is not None and lengths.dtype == torch.int64)
+    args.B, args.T, args.D = x.shape
+    args.logit, args.mix, args.reverse = how
+    return args
+
+
+class _LinearScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, h0, lengths, logit, mix, reverse):
+        B, T, D = x.shape
+        how = (logit, mix, reverse)
+        if x.device.type == "cpu":
+            h, last, _ = _forward_torch(x, gate, h0, _lengths(lengths, B, T), *how)
+        else:
+            entry = native("pda_scan_fwd")
+            h = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
+            last = torch.empty(B, D, dtype=torch.float32, device=x.device)
+            args = _fill(_Args(), x, gate, h0, lengths, how)
+            args.h, args.last = ptr(h), ptr(last)
+            with on_device(x):
+                launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "linear_scan")
+        ctx.save_for_backward(x, gate, h0, lengths)
+        ctx.how = how
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dlast):
+        x, gate, h0, lengths = ctx.saved_tensors
+        none = (None,) * 7
+        if dh is None and dlast is None:
+            return none
+        B, T, D = x.shape
+        if x.device.type == "cpu":
+            dx, dg, dh0 = _backward_torch(x, gate, h0, _lengths(lengths, B, T), *ctx.how, dh, dlast)
+        else:
+            entry = native("pda_scan_bwd")
+            dlast = dlast.contiguous() if dlast is not None else None
+            dx = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
+            dg, dh0 = torch.empty_like(dx), torch.empty(B, D, dtype=torch.float32, device=x.device)
+            hist = torch.empty(B, T, D, dtype=torch.float32, device=x.device)
+            args = _fill(_Args(), x, gate, h0, lengths, ctx.how)
+            args.dh, args.dlast, args.dx, args.dg, args.dh0, args.hist = map(ptr, (dh, dlast, dx, dg, dh0, hist))
+            if dh is not None:
+                args.ds[:] = dh.stride()
+            with on_device(x):
+                launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "linear_scan backward")
+        return dx, dg, (dh0 if h0 is not None else None), None, None, None, None
+
+
+def _check_gates(gates):
+    if gates not in GATES:
+        raise ValueError("gates must be one of %s, not %r" % ("|".join(GATES), gates))
+    return int(gates == "logit")
+
+
+def _same(t, what, like, dtype=None):
+    dtype = like.dtype if dtype is None else dtype
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != like.device:
+        raise ValueError("%s must be a %s tensor on %s" % (what, dtype, like.device))
+
+
+def linear_scan(x, gate, h0=None, gates="decay", mix=False, reverse=False, lengths=None):
+    """-> (h, last): h_t = a_t h_{t-1} + u_t along dimension 1.
+
+    x, gate    [B, T, D] (or [B, T]: one channel), float32, bfloat16 or float16, of one type; any strides, so a gate
+               shared by steps or channels may be passed as an expanded view (its gradient is summed by autograd)
+    gates      "decay": a = gate  |  "logit": a = sigmoid(gate)
+    mix        False: u = x  |  True: u = (1 - a) x (a leaky average)
+    h0         [B, D] (or [B]) float32 state in front of the first step, None = 0
+    reverse    run from the last step to the first (discounted returns: gate = gamma, 0 behind an episode's end)
+    lengths    [B] int32 / int64: sequence b is its first lengths[b] steps (clamped to 0 .. T; reverse starts at the last
+               of them); the other steps are not read, their h and gradients are 0
+
+    h has x's shape and type and is contiguous; last is the float32 state behind the last step (h0 where a length is 0).
+    The state is 32 bits wide throughout.  Gradients flow from h and last to x, gate and h0 (not twice).  Decay gates are
+    meant to be within [-1, 1]; with larger ones, products of gates over a few hundred steps can overflow 32 bits and the
+    result is then inf or NaN even where the exact one is finite."""
+    check_floating(x, "x")
+    logit = _check_gates(gates)
+    if x.dim() not in (2, 3):
+        raise ValueError("x must be [B, T, D] or [B, T], not shape %s" % (tuple(x.shape),))
+    _same(gate, "gate", x)
+    if gate.shape != x.shape:
+        raise ValueError("gate has shape %s, x %s (expand a shared gate)" % (tuple(gate.shape), tuple(x.shape)))
+    state = (x.shape[0],) + tuple(x.shape[2:])
+    if h0 is not None:
+        _same(h0, "h0", x, torch.float32)
+        if tuple(h0.shape) != state:
+            raise ValueError("h0 has shape %s, expected %s" % (tuple(h0.shape), state))
+    if lengths is not None:
+        check_int(lengths, "lengths", x.shape[:1], x.device)
+        lengths = lengths.contiguous()
+    flat = x.dim() == 2
+    if flat:
+        x, gate, h0 = x.unsqueeze(2), gate.unsqueeze(2), h0.unsqueeze(1) if h0 is not None else None
+    if x.shape[0] * x.shape[2] >= 1 << 31 or x.shape[1] >= 1 << 31:
+        raise ValueError("x of shape %s is too large" % (tuple(x.shape),))
+    h0 = h0.contiguous() if h0 is not None else None
+    h, last = _LinearScan.apply(x, gate, h0, lengths, logit, int(bool(mix)), int(bool(reverse)))
+    return (h.squeeze(2), last.squeeze(1)) if flat else (h, last)
+
+
+def _overlap(a, b):
+    """Whether the address ranges of two tensors meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in
+                                                                                zip(t.shape, t.stride())))) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
+@torch.no_grad()
+def linear_scan_step(x, gate, state, gates="decay", mix=False, state_out=None):
+    """One step of `linear_scan` for every request of a batch: h = a state + u, returned in x's type and written in 32 bits
+    to `state` itself, or to state_out, a second buffer (memory that overlaps state, x or gate otherwise than as the same view is refused).
+
+    x, gate [B, D] of one type, state float32 [B, D]; any strides, but no element of the written buffer may be shared
+    (an expanded view is refused).  No gradient."""
+    check_floating(x, "x")
+    logit = _check_gates(gates)
+    if x.dim() != 2:
+        raise ValueError("x must be [B, D], not shape %s" % (tuple(x.shape),))
+    _same(gate, "gate", x)
+    out = state if state_out is None else state_out
+    for t, what in ((state, "state"), (out, "state_out")):
+        _same(t, what, x, torch.float32)
+    for t, what in ((gate, "gate"), (state, "state"), (out, "state_out")):
+        if t.shape != x.shape:
+            raise ValueError("%s has shape %s, x %s" % (what, tuple(t.shape), tuple(x.shape)))
+    B, D = x.shape
+    if not out.is_contiguous():
+        (s0, n0), (s1, n1) = sorted(zip(out.stride(), out.shape))
+        if (n0 > 1 and s0 == 0) or (n1 > 1 and s1 < s0 * (n0 - 1) + 1):
+            raise ValueError("the written state shares elements between requests or channels (strides %s)" % (out.stride(),))
+    for t, what in ((state, "state"), (x, "x"), (gate, "gate")):
+        if not (t.data_ptr() == out.data_ptr() and t.stride() == out.stride() and t.dtype == out.dtype) and _overlap(t, out):
+            raise ValueError("the written state overlaps %s in memory without being the same view" % what)
+    if x.device.type == "cpu":
+        h = _advance(state, x, gate, logit, mix)
+        out.copy_(h)
+        return h.to(x.dtype)
+    entry = native("pda_scan_step")
+    h = torch.empty(B, D, dtype=x.dtype, device=x.device)
+    args = _StepArgs(ptr(x), ptr(gate), ptr(state), ptr(out), ptr(h))
+    args.xs[:], args.gs[:], args.ss[:], args.os[:] = x.stride(), gate.stride(), state.stride(), out.stride()
+    args.B, args.D, args.logit, args.mix = B, D, logit, int(bool(mix))
+    with on_device(x):
+        launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "linear_scan_step")
+    return h
