@@ -22,6 +22,11 @@ ARCH = "gfx950"
 # undefined behaviour.
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-fno-gpu-rdc", "-fvisibility=hidden",
          "-Wall", "-Wno-unused-function", "-ffast-math", "-fno-finite-math-only"]
+# Added for the named sources: no packed fp32 instructions, some of whose forms have given wrong results now and then
+# (hipcc's host pass warns that it does not know the feature).  The learner's kernels keep the flags they were measured
+# with: without packed instructions their sums round elsewhere and the steps are 1 % slower (10.56 k -> 10.44 k updates/s).
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+SOURCE_FLAGS = {"logprob.hip": NO_PACKED_FP32, "scan.hip": NO_PACKED_FP32, "dropout.hip": NO_PACKED_FP32}
 
 
 def _hipcc():
@@ -58,10 +63,11 @@ def build(force=False, verbose=False, extra_flags=()):
         objs.append(obj)
         # (the flags are part of the recipe: an object built with other flags is stale too)
         stamp = obj + ".flags"
-        flags = " ".join(FLAGS + list(extra_flags))
+        own = FLAGS + SOURCE_FLAGS.get(os.path.basename(src), []) + list(extra_flags)
+        flags = " ".join(own)
         same_flags = os.path.exists(stamp) and open(stamp).read() == flags
         if force or not same_flags or _stale(obj, [src] + headers):
-            jobs.append([hipcc] + FLAGS + list(extra_flags) + ["-c", src, "-o", obj])
+            jobs.append([hipcc] + own + ["-c", src, "-o", obj])
             LAST_REPORT[os.path.basename(src)] = "compiled"
             if os.path.exists(stamp):
                 os.remove(stamp)
@@ -81,7 +87,7 @@ def build(force=False, verbose=False, extra_flags=()):
         list(pool.map(run, jobs))
     for cmd in jobs:
         with open(cmd[-1] + ".flags", "w") as fh:
-            fh.write(" ".join(FLAGS + list(extra_flags)))
+            fh.write(" ".join(cmd[1:-4]))
     LAST_REPORT["link"] = "linked" if (force or jobs or _stale(LIB, objs)) else "reused"
     if force or jobs or _stale(LIB, objs):
         tmp = LIB + ".tmp%d" % os.getpid()
