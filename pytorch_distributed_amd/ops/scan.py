@@ -17,9 +17,9 @@ _vp, _i64, _int = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
 
 class _Args(ctypes.Structure):      # mirrors ScanArgs in csrc/scan.hip
     _fields_ = [("x", _vp), ("gate", _vp), ("dh", _vp), ("xs", _i64 * 3), ("gs", _i64 * 3), ("ds", _i64 * 3), ("h0", _vp),
-                ("dlast", _vp), ("lengths", _vp), ("len64", _int), ("h", _vp), ("last", _vp), ("hist", _vp), ("dx", _vp),
-                ("dg", _vp), ("dh0", _vp), ("B", _int), ("T", _int), ("D", _int), ("logit", _int), ("mix", _int),
-                ("reverse", _int)]
+                ("dlast", _vp), ("lengths", _vp), ("len64", _int), ("h", _vp), ("last", _vp), ("carry", _vp),
+                ("sums", _vp), ("dx", _vp), ("dg", _vp), ("dh0", _vp), ("B", _int), ("T", _int), ("D", _int),
+                ("logit", _int), ("mix", _int), ("reverse", _int), ("chunks", _int)]
 
 
 class _StepArgs(ctypes.Structure):  # mirrors ScanStepArgs
@@ -83,6 +83,14 @@ def _backward_torch(x, gate, h0, n, logit, mix, reverse, dh, dlast):
     return dx, dg, carry
 
 
+def _plan(x):
+    """-> (tiles, chunks): how the kernels cut x's steps (csrc/scan.hip scan_plan)"""
+    out = (ctypes.c_int * 2)()
+    B, T, D = x.shape
+    native("pda_scan_plan")(B, T, D, TYPE_CODES[x.dtype], ctypes.byref(out, 0), ctypes.byref(out, 4))
+    return out[0], out[1]
+
+
 def _lengths(lengths, B, T):
     return torch.full((B,), T) if lengths is None else lengths.long().clamp(0, T)
 
@@ -101,6 +109,7 @@ class _LinearScan(torch.autograd.Function):
     def forward(ctx, x, gate, h0, lengths, logit, mix, reverse):
         B, T, D = x.shape
         how = (logit, mix, reverse)
+        carry = None
         if x.device.type == "cpu":
             h, last, _ = _forward_torch(x, gate, h0, _lengths(lengths, B, T), *how)
         else:
@@ -108,10 +117,16 @@ class _LinearScan(torch.autograd.Function):
             h = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
             last = torch.empty(B, D, dtype=torch.float32, device=x.device)
             args = _fill(_Args(), x, gate, h0, lengths, how)
-            args.h, args.last = ptr(h), ptr(last)
+            tiles, args.chunks = _plan(x)
+            if any(ctx.needs_input_grad):
+                carry = torch.empty(B, tiles, D, dtype=torch.float32, device=x.device)
+            if args.chunks > 1:
+                sums = torch.empty(B, args.chunks, 2, D, dtype=torch.float32, device=x.device)
+                args.sums = ptr(sums)
+            args.h, args.last, args.carry = ptr(h), ptr(last), ptr(carry)
             with on_device(x):
                 launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "linear_scan")
-        ctx.save_for_backward(x, gate, h0, lengths)
+        ctx.save_for_backward(x, gate, h0, lengths, carry)
         ctx.how = how
         ctx.set_materialize_grads(False)
         return h, last
@@ -119,7 +134,7 @@ class _LinearScan(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dlast):
-        x, gate, h0, lengths = ctx.saved_tensors
+        x, gate, h0, lengths, carry = ctx.saved_tensors
         none = (None,) * 7
         if dh is None and dlast is None:
             return none
@@ -131,9 +146,12 @@ class _LinearScan(torch.autograd.Function):
             dlast = dlast.contiguous() if dlast is not None else None
             dx = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
             dg, dh0 = torch.empty_like(dx), torch.empty(B, D, dtype=torch.float32, device=x.device)
-            hist = torch.empty(B, T, D, dtype=torch.float32, device=x.device)
             args = _fill(_Args(), x, gate, h0, lengths, ctx.how)
-            args.dh, args.dlast, args.dx, args.dg, args.dh0, args.hist = map(ptr, (dh, dlast, dx, dg, dh0, hist))
+            args.chunks = _plan(x)[1]
+            if args.chunks > 1:
+                sums = torch.empty(B, args.chunks, 2, D, dtype=torch.float32, device=x.device)
+                args.sums = ptr(sums)
+            args.dh, args.dlast, args.dx, args.dg, args.dh0, args.carry = map(ptr, (dh, dlast, dx, dg, dh0, carry))
             if dh is not None:
                 args.ds[:] = dh.stride()
             with on_device(x):
