@@ -23,7 +23,8 @@ class _Args(ctypes.Structure):      # mirrors LogprobArgs in csrc/logprob.hip
     _fields_ = [("logits", _vp), ("ld", _i64), ("rows", _i64), ("vocab", ctypes.c_int), ("tokens", _vp),
                 ("tok64", ctypes.c_int), ("ignore", _i64), ("inv_t", ctypes.c_float), ("top_k", ctypes.c_int),
                 ("logprob", _vp), ("entropy", _vp), ("lse", _vp), ("stat_m", _vp), ("stat_ls", _vp), ("top_lp", _vp),
-                ("top_id", _vp), ("d_lp", _vp), ("d_ent", _vp), ("d_lse", _vp), ("d_logits", _vp)]
+                ("top_id", _vp), ("d_lp", _vp), ("d_ent", _vp), ("d_lse", _vp), ("d_logits", _vp),
+                ("splits", ctypes.c_int), ("part_stat", _vp), ("part_top", _vp)]
 
 
 def _forward_torch(x, tokens, inv_t, top_k, ignore):
@@ -86,6 +87,11 @@ class _TokenLogprobs(torch.autograd.Function):
             args = _fill(_Args(), x, tokens, inv_t, ignore)
             args.logprob, args.entropy, args.lse, args.stat_m, args.stat_ls = map(ptr, (lp, ent, lse, m, ls))
             args.top_lp, args.top_id, args.top_k = ptr(top), ptr(ids), top_k
+            args.splits = native("pda_logprob_splits")(_i64(n), x.shape[1], top_k)
+            if args.splits > 1:     # long rows in parts, joined by a second launch
+                stat = torch.empty(n, args.splits, 4, dtype=torch.float32, device=x.device)
+                keys = torch.empty(n, args.splits, top_k, dtype=torch.int64, device=x.device)
+                args.part_stat, args.part_top = ptr(stat), ptr(keys)
             with on_device(x):
                 launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "token_logprobs")
         ctx.save_for_backward(x, tokens, m, ls, ent)
