@@ -4,7 +4,9 @@
 //   logprob = (x_t - m) / T - log s,   entropy = log s - u / s,   logsumexp = m / T + log s
 //   dx_i = (p_i (dlse - dlp - dent (logp_i + entropy)) + dlp [i = t]) / T,   p_i = exp(logp_i)
 //
-// (m, log s) is what the forward pass keeps for the backward pass: their sum would round p by |lse| 2^-24.
+// Exponents are formed as 2^(x c - r), c = log2(e) / T, r = m c rounded: one fused multiply-add per value.  r's rounding
+// is common to all values of a row and cancels, because s is taken relative to r and logp = (x c - r) - log2 s.
+// (m, log2 s) is what the forward pass keeps for the backward pass: their sum would round p by |lse| 2^-24.
 // A logit of -inf is a masked token: p = 0, no share in the entropy, gradient 0.  A row with nothing but -inf: logprob
 // and logsumexp -inf, entropy 0, gradient 0.  An ignored row is not read: 0 everywhere, alternatives -1.
 // A token outside the vocabulary gives NaN (log-probability and gradient row) and reads nothing.
@@ -14,9 +16,9 @@
 struct LogprobArgs {
     const void* logits; long long ld; long long rows; int vocab;
     const void* tokens; int tok64; long long ignore;
-    float inv_t; int top_k;
+    float inv_t, c; int top_k;                          // 1 / T, log2(e) / T
     float* logprob; float* entropy; float* lse;         // [rows]
-    float* stat_m; float* stat_ls;                      // [rows], for the backward pass
+    float* stat_m; float* stat_l2;                      // [rows]: m, log2 s, for the backward pass
     float* top_lp; long long* top_id;                   // [rows][top_k]
     // backward
     const float* d_lp; const float* d_ent; const float* d_lse;  // [rows], any may be null
@@ -49,15 +51,22 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
     return v;
 }
 
-// softmax statistics of a part of a row: running maximum m, and s, u relative to it, with u in units of log 2:
-// s = sum 2^d, u = sum 2^d d, d = (x - m) c, c = log2(e) / T
+// softmax statistics of a part of a row: its maximum m, and relative to r = m c rounded: s = sum 2^d, u = sum 2^d d,
+// d = x c - r
 struct LpStat { float m, s, u; };
 #define LP_LN2 0.693147180559945309f
-#define LP_LOG2E 1.44269504088896341f
+// The rounding of r is at most |r| 2^-24: below this bound 2^(its rounding) stays near 1.  Rows beyond it (logits of more
+// than 7e6 T, masks of the type's lowest value in every place) are walked once more with d = (x - m) c.
+#define LP_NEAR 1.0e7f
 __device__ __forceinline__ float lp_exp2(float d) { return __builtin_amdgcn_exp2f(d); }
+__device__ __forceinline__ float lp_ref(float m, float c) {
+    float r = m * c;
+    asm("" : "+v"(r));          // r is this rounded product wherever it is used: no contraction into an fma
+    return r;
+}
 // `st` seen from the maximum m >= st.m (no part of it may turn into 0 * inf: the shift is cut off where 2^shift is 0)
 __device__ __forceinline__ LpStat lp_shift(LpStat st, float m, float c) {
-    const float d = st.m == m ? 0.f : fmaxf((st.m - m) * c, -1.0e20f), e = lp_exp2(d);
+    const float d = st.m == m ? 0.f : fmaxf(lp_ref(st.m, c) - lp_ref(m, c), -1.0e20f), e = lp_exp2(d);
     return LpStat{m, st.s * e, e * __builtin_fmaf(d, st.s, st.u)};
 }
 __device__ __forceinline__ LpStat lp_merge(LpStat a, LpStat b, float c) {
@@ -70,19 +79,20 @@ __device__ __forceinline__ LpStat lp_merge(LpStat a, LpStat b, float c) {
 template <int NX>
 __device__ __forceinline__ void lp_add(LpStat& st, const float (&x)[NX], float bm, float c) {
     st = lp_shift(st, fmaxf(st.m, bm), c);
-    const float m = st.m == -INFINITY ? 0.f : st.m;
+    const float r = st.m == -INFINITY ? 0.f : lp_ref(st.m, c);
     float s = 0.f, u = 0.f;
 #pragma unroll
     for (int i = 0; i < NX; ++i) {
-        const float d = (x[i] - m) * c, e = lp_exp2(d);
-        s += e;                                             // (NaN for a NaN, and for +inf - +inf)
+        const float d = __builtin_fmaf(x[i], c, -r), e = lp_exp2(d);
+        s += e;                                             // (NaN for a NaN)
         u = __builtin_fmaf(e, fmaxf(d, -1000.f), u);        // (0 for -inf)
     }
     st.s += s;
     st.u += u;
 }
+// over groups of G lanes
 template <int G>
-__device__ __forceinline__ LpStat lp_across(LpStat st, float c) {   // over groups of G lanes
+__device__ __forceinline__ LpStat lp_across(LpStat st, float c) {
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1)
         st = lp_merge(st, LpStat{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.u, o, 64)}, c);
@@ -91,38 +101,80 @@ __device__ __forceinline__ LpStat lp_across(LpStat st, float c) {   // over grou
 
 __device__ __forceinline__ void lp_ignored_row(const LogprobArgs& p, long long row) {
     p.logprob[row] = 0.f; p.entropy[row] = 0.f; p.lse[row] = 0.f;
-    p.stat_m[row] = 0.f; p.stat_ls[row] = 0.f;
+    p.stat_m[row] = 0.f; p.stat_l2[row] = 0.f;
     for (int k = 0; k < p.top_k; ++k) { p.top_lp[row * p.top_k + k] = 0.f; p.top_id[row * p.top_k + k] = -1; }
 }
-__device__ __forceinline__ bool lp_empty(LpStat st) { return st.m == -INFINITY && st.s == 0.f; }
-__device__ __forceinline__ bool lp_not_a_number(LpStat st) { return st.m == INFINITY || st.s != st.s; }
-__device__ __forceinline__ float lp_log_sum(LpStat st) { return lp_not_a_number(st) ? __builtin_nanf("") : __logf(st.s); }
-template <typename T>
-__device__ __forceinline__ void lp_finish_row(const LogprobArgs& p, long long row, long long tok, LpStat st) {
-    const T* x = (const T*)p.logits + row * p.ld;
-    const bool empty = lp_empty(st);
-    const float ls = empty ? 0.f : lp_log_sum(st);
-    float lp = __builtin_nanf("");
-    if (tok >= 0 && tok < p.vocab) lp = empty ? -INFINITY : (to_f32(x[tok]) - st.m) * p.inv_t - ls;
-    p.logprob[row] = lp;
-    p.entropy[row] = empty ? 0.f : ls - st.u / st.s * LP_LN2;
-    p.lse[row] = empty ? -INFINITY : st.m * p.inv_t + ls;
-    p.stat_m[row] = st.m;
-    p.stat_ls[row] = ls;
+
+// What the row's values become.  NEAR: d = x c - r; otherwise d = (x - m) c, for rows whose m c leaves 32 bits, and for
+// short rows, which cost nothing either way.
+struct LpRow {
+    float m, r, c, l2; bool near, empty;
+    __device__ __forceinline__ LpRow(float m_, float l2_, float c_, bool short_row) : m(m_), c(c_), l2(l2_) {
+        r = lp_ref(m, c);
+        near = !short_row && fabsf(r) < LP_NEAR;
+        empty = m == -INFINITY && l2 == l2;     // nothing but -inf
+    }
+    __device__ __forceinline__ float log2p(float x) const { return (near ? __builtin_fmaf(x, c, -r) : (x - m) * c) - l2; }
+    __device__ __forceinline__ float logp(float x, float inv_t) const {
+        if (empty) return -INFINITY;
+        const float v = log2p(x) * LP_LN2;      // (x c may leave 32 bits where x / T does not)
+        return v == -INFINITY && x > -INFINITY ? (x - m) * inv_t - l2 * LP_LN2 : v;
+    }
+};
+// s = 0 for a row of nothing but -inf; NaN where the row holds NaN or +inf
+__device__ __forceinline__ float lp_log2_sum(LpStat st) {
+    if (st.m == INFINITY || st.s != st.s) return __builtin_nanf("");
+    return st.s == 0.f ? 0.f : __builtin_amdgcn_logf(st.s);
 }
 template <typename T>
-__device__ __forceinline__ void lp_put_alternative(const LogprobArgs& p, long long row, int k, uint64_t key, LpStat st, float ls) {
+__device__ __forceinline__ void lp_finish_row(const LogprobArgs& p, long long row, long long tok, LpStat st, const LpRow& q) {
+    const T* x = (const T*)p.logits + row * p.ld;
+    p.logprob[row] = tok >= 0 && tok < p.vocab ? q.logp(to_f32(x[tok]), p.inv_t) : __builtin_nanf("");
+    p.entropy[row] = q.empty ? 0.f : (q.l2 - st.u / st.s) * LP_LN2;
+    p.lse[row] = q.empty ? -INFINITY : q.near ? (q.r + q.l2) * LP_LN2 : __builtin_fmaf(q.m, p.inv_t, q.l2 * LP_LN2);
+    p.stat_m[row] = st.m;
+    p.stat_l2[row] = q.l2;
+}
+template <typename T>
+__device__ __forceinline__ void lp_put_alternative(const LogprobArgs& p, long long row, int k, uint64_t key, const LpRow& q) {
     const int id = lp_key_index(key);
-    const float x = to_f32(((const T*)p.logits + row * p.ld)[id]);
     p.top_id[row * p.top_k + k] = id;
-    p.top_lp[row * p.top_k + k] = lp_empty(st) ? -INFINITY : (x - st.m) * p.inv_t - ls;
+    p.top_lp[row * p.top_k + k] = q.logp(to_f32(((const T*)p.logits + row * p.ld)[id]), p.inv_t);
 }
 
-// The alternatives of a row that holds NaN, by top_k walks over it (float comparisons cannot order those): whole workgroup
+// Rows that the running statistics cannot take: nothing but -inf, NaN, +inf, or |m c| beyond LP_NEAR.  Whole workgroup, two walks and one more for each alternative.
 template <typename T>
-__device__ void lp_walk_top(const LogprobArgs& p, long long row, LpStat st, float ls, uint64_t* best) {
+__device__ __forceinline__ void lp_walk_row(const LogprobArgs& p, long long row, long long tok, LpStat* part, uint64_t* best) {
     const T* x = (const T*)p.logits + row * p.ld;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    float m = -INFINITY, bad = 0.f;
+    for (int i = tid; i < p.vocab; i += 256) {
+        const float v = to_f32(x[i]);
+        m = fmaxf(m, v);
+        if (v != v) bad = v;
+    }
+    m = wave_max(m);
+    bad = wave_sum(bad);
+    __syncthreads();                // (earlier reads of part[] and best[])
+    if (lane == 0) part[wave] = LpStat{m, bad, 0.f};
+    __syncthreads();
+    m = fmaxf(fmaxf(part[0].m, part[1].m), fmaxf(part[2].m, part[3].m));
+    bad = part[0].s + part[1].s + part[2].s + part[3].s;
+    float s = bad, u = 0.f;
+    if (m > -INFINITY)
+        for (int i = tid; i < p.vocab; i += 256) {
+            const float d = (to_f32(x[i]) - m) * p.c, e = lp_exp2(d);
+            s += e;
+            u += e > 0.f ? e * d : 0.f;
+        }
+    s = wave_sum(s);
+    u = wave_sum(u);
+    __syncthreads();
+    if (lane == 0) part[wave] = LpStat{m, s, u};
+    __syncthreads();
+    const LpStat st{m, (part[0].s + part[1].s) + (part[2].s + part[3].s), (part[0].u + part[1].u) + (part[2].u + part[3].u)};
+    LpRow q(m, lp_log2_sum(st), p.c, true);
+    if (tid == 0) lp_finish_row<T>(p, row, tok, st, q);
     uint64_t last = ~0ull;
     for (int k = 0; k < p.top_k; ++k) {
         uint64_t b = 0;
@@ -132,20 +184,24 @@ __device__ void lp_walk_top(const LogprobArgs& p, long long row, LpStat st, floa
         }
         b = wave_max_u64(b);
         __syncthreads();            // (the previous round's reads of best[])
-        if ((tid & 63) == 0) best[tid >> 6] = b;
+        if (lane == 0) best[wave] = b;
         __syncthreads();
         last = best[0];
         for (int w = 1; w < 4; ++w) last = best[w] > last ? best[w] : last;
-        if (tid == 0) lp_put_alternative<T>(p, row, k, last, st, ls);
+        if (tid == 0) lp_put_alternative<T>(p, row, k, last, q);
     }
     __syncthreads();
 }
-// The top_k largest of n distinct keys in LDS, by counting what is above each: whole workgroup
+__device__ __forceinline__ bool lp_ordinary(LpStat st, float c) {
+    return st.s > 0.f && st.s < INFINITY && fabsf(lp_ref(st.m, c)) < LP_NEAR;
+}
+// The top_k largest of n distinct keys (0: none) in LDS, by counting what is above each: whole workgroup
 template <typename F>
 __device__ __forceinline__ void lp_rank(const uint64_t* keys, int n, int top_k, F put) {
     for (int i = threadIdx.x; i < n; i += 256) {
         const uint64_t mine = keys[i];
         int above = 0;
+#pragma unroll 8
         for (int j = 0; j < n; ++j) above += keys[j] > mine ? 1 : 0;
         if (above < top_k && mine != 0) put(above, mine);
     }
@@ -155,7 +211,6 @@ __device__ __forceinline__ void lp_rank(const uint64_t* keys, int n, int top_k, 
 template <typename T, int E, int G>
 __global__ __launch_bounds__(256) void logprob_short_kernel(LogprobArgs p) {
     const int lane = threadIdx.x & 63, l = lane & (G - 1);
-    const float c = p.inv_t * LP_LOG2E;
     const long long step = (long long)gridDim.x * (256 / G);
     // (every lane of a wave takes every round: the shuffles want them all)
     for (long long r0 = (long long)blockIdx.x * (256 / G); r0 < p.rows; r0 += step) {
@@ -164,23 +219,31 @@ __global__ __launch_bounds__(256) void logprob_short_kernel(LogprobArgs p) {
         const long long tok = on ? lp_token(p, row) : p.ignore;
         const bool live = on && tok != p.ignore;
         const T* x = (const T*)p.logits + (live ? row : 0) * p.ld;
-        float xs[E], bm = -INFINITY;
+        float xs[E], m = -INFINITY, bad = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int i = l + e * G;
             xs[e] = live && i < p.vocab ? to_f32(x[i]) : -INFINITY;
-            bm = fmaxf(bm, xs[e]);
+            m = fmaxf(m, xs[e]);
+            if (xs[e] != xs[e]) bad = xs[e];
         }
 #pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) bm = fmaxf(bm, __shfl_xor(bm, o, 64));
-        LpStat st{-INFINITY, 0.f, 0.f};
-        lp_add<E>(st, xs, bm, c);
-        st = lp_across<G>(st, c);
+        for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        float s = bad, u = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float d = m == -INFINITY ? -INFINITY : (xs[e] - m) * p.c, ex = lp_exp2(d);
+            s += ex;
+            u += ex > 0.f ? ex * d : 0.f;
+        }
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); u += __shfl_xor(u, o, 64); }
+        const LpStat st{m, s, u};
+        const LpRow q(m, lp_log2_sum(st), p.c, true);
         if (l == 0 && on) {
-            if (live) lp_finish_row<T>(p, row, tok, st);
+            if (live) lp_finish_row<T>(p, row, tok, st, q);
             else lp_ignored_row(p, row);
         }
-        const float ls = lp_log_sum(st);
         uint64_t last = ~0ull;
         for (int k = 0; k < p.top_k; ++k) {
             uint64_t b = 0;
@@ -196,23 +259,72 @@ __global__ __launch_bounds__(256) void logprob_short_kernel(LogprobArgs p) {
                 b = t > b ? t : b;
             }
             last = b;
-            if (l == 0 && live) lp_put_alternative<T>(p, row, k, last, st, ls);
+            if (l == 0 && live) lp_put_alternative<T>(p, row, k, last, q);
         }
     }
 }
 
 // ---- long rows ---------------------------------------------------------------------------------------------------------
-// A workgroup reads a row (or one of its splits) once, in 16-byte loads, four in flight per thread.  Each thread keeps
-// running statistics, shifted once per 32 or 16 values.  The alternatives: each wave keeps its best keys sorted over its
-// lanes.  A value is looked at again only if it passes the wave's k-th best, which the first batch sets to the k-th largest
-// of the lanes' maxima; a wave of n values then inserts about k (2 + ln(n / 2048)) of them, each by a ballot and a shift.
+__device__ __forceinline__ uint64_t lp_lane(uint64_t v, int lane) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+__device__ __forceinline__ uint64_t lp_next_lane(uint64_t v) {      // lane i gets lane i - 1's (0x138: wave_shr by one)
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), 0x138, 0xf, 0xf, false);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)v, 0x138, 0xf, 0xf, false);
+    return ((uint64_t)hi << 32) | lo;
+}
+// A wave's best keys, sorted over its lanes, and what a value has to reach (`strict`: to exceed) to come among them.
+struct LpList {
+    uint64_t key; float lim; bool strict, full;
+    __device__ __forceinline__ LpList() : key(0), lim(-INFINITY), strict(false), full(false) {}
+    __device__ __forceinline__ bool passes(float v) const { return strict ? v > lim : v >= lim; }
+    // k-th largest of the lanes' t: at least k values of the first batch reach it
+    __device__ __forceinline__ void first_limit(float t, int k) {
+        const int lane = threadIdx.x & 63;
+        int above = 0;
+#pragma unroll 16
+        for (int o = 0; o < 64; ++o) {
+            const float other = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, t), o));
+            above += (other > t || (other == t && o < lane)) ? 1 : 0;
+        }
+        const uint64_t who = __ballot(above == k - 1);
+        if (who) lim = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, t), __builtin_ctzll(who)));
+    }
+    // the lanes of `todo` offer a key each (all lanes take part)
+    __device__ __forceinline__ void insert(uint64_t todo, uint64_t mine, int k) {
+        const int lane = threadIdx.x & 63;
+        while (todo) {
+            const int src = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const uint64_t q = lp_lane(mine, src);
+            const int pos = __builtin_popcountll(__ballot(key > q));
+            if (pos >= k) continue;
+            const uint64_t up = lp_next_lane(key);
+            key = lane < pos ? key : (lane == pos ? q : up);
+        }
+        const uint64_t kth = lp_lane(key, k - 1);
+        if (kth == 0) return;
+        uint32_t b = (uint32_t)(kth >> 32);
+        b = (b & 0x80000000u) ? (b & 0x7fffffffu) : ~b;
+        const float v = __builtin_bit_cast(float, b);
+        if (!full || v > lim) { lim = v; strict = false; }      // equal values of this batch may have lower indices
+        full = true;
+    }
+};
+
+// A workgroup reads a row (or one of its splits) once, in 16-byte loads, the next four in flight while four are worked on.
+// Each thread keeps running statistics, shifted once per 32 or 16 values.  The alternatives: each wave keeps its best keys
+// sorted over its lanes.  A value is looked at again only if it passes the wave's k-th best, which the first batch sets to
+// the k-th largest of the lanes' maxima; a wave of n values then inserts about k (2 + ln(n / 2048)) of them, each by a
+// ballot and a shift by one lane.
 template <typename T>
 __global__ __launch_bounds__(256) void logprob_long_kernel(LogprobArgs p) {
     constexpr int VEC = 16 / sizeof(T), U = 4, NX = U * VEC;
     __shared__ LpStat part[4];
     __shared__ uint64_t keys[4 * LP_MAX_TOP];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const float c = p.inv_t * LP_LOG2E;
+    const float c = p.c;
     const long long units = p.rows * p.splits;
     for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const long long row = unit / p.splits;
@@ -227,88 +339,65 @@ __global__ __launch_bounds__(256) void logprob_long_kernel(LogprobArgs p) {
         const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), p.vocab);
         const int nvec = (p.vocab - head) / VEC, tail = (p.vocab - head) - nvec * VEC;
         const int per = (nvec + p.splits - 1) / p.splits, v0 = min(split * per, nvec), v1 = min(v0 + per, nvec);
+        const vec16<T>* xv = reinterpret_cast<const vec16<T>*>(x + head);
         LpStat st{-INFINITY, 0.f, 0.f};
-        uint64_t list = 0;                  // lane i: the wave's i-th best key so far
-        float lim = -INFINITY;              // what a value has to reach (or, `strict`, to exceed) to get into it
-        bool strict = false, filled = false;
-        auto offer = [&](float v, int index, bool valid) {
-            const bool pass = valid && (strict ? v > lim : v >= lim);
-            uint64_t todo = __ballot(pass);
-            if (todo == 0) return;
-            const uint64_t key = lp_key(v, index);
-            while (todo) {
-                const int src = __builtin_ctzll(todo);
-                todo &= todo - 1;
-                const uint64_t k = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), src) << 32) |
-                                   (uint32_t)__builtin_amdgcn_readlane((int)key, src);
-                const uint64_t above = __ballot(list > k);
-                const int pos = __builtin_popcountll(above);
-                if (pos >= p.top_k) continue;
-                const uint64_t up = __shfl_up((unsigned long long)list, 1, 64);
-                list = lane < pos ? list : (lane == pos ? k : up);
-            }
-            const uint64_t kth = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(list >> 32), p.top_k - 1) << 32) |
-                                 (uint32_t)__builtin_amdgcn_readlane((int)list, p.top_k - 1);
-            if (kth != 0) {
-                uint32_t b = (uint32_t)(kth >> 32);
-                b = (b & 0x80000000u) ? (b & 0x7fffffffu) : ~b;
-                const float v = __builtin_bit_cast(float, b);
-                if (!filled || v > lim) { lim = v; strict = false; }
-                filled = true;
-            }
-        };
-        bool first = true;
+        LpList list;
+        vec16<T> cur[U], nxt[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int v = v0 + u * 256 + tid;
+            if (v < v1) cur[u] = xv[v];
+        }
         for (int b = v0; b < v1; b += 256 * U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int v = b + (U + u) * 256 + tid;
+                if (v < v1) nxt[u] = xv[v];
+            }
             float xs[NX], bm = -INFINITY;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int v = b + u * 256 + tid;
-                if (v < v1) {
-                    const vec16<T> q = *reinterpret_cast<const vec16<T>*>(x + head + (long long)v * VEC);
+                const bool in = b + u * 256 + tid < v1;
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) xs[u * VEC + j] = to_f32(q.e[j]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) xs[u * VEC + j] = -INFINITY;
-                }
+                for (int j = 0; j < VEC; ++j) xs[u * VEC + j] = in ? to_f32(cur[u].e[j]) : -INFINITY;
             }
 #pragma unroll
             for (int i = 0; i < NX; ++i) bm = fmaxf(bm, xs[i]);
             lp_add<NX>(st, xs, bm, c);
-            if (p.top_k == 0) continue;
-            if (first) {        // the k-th largest of the lanes' maxima: k values reach it
-                first = false;
-                float t = bm;
-                int above = 0;
-                for (int o = 0; o < 64; ++o) {
-                    const float other = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, t), o));
-                    above += (other > t || (other == t && o < lane)) ? 1 : 0;
+            if (p.top_k > 0) {
+                if (b == v0) list.first_limit(bm, p.top_k);
+                else if (list.full) list.strict = true;     // an equal value of a later batch has a higher index
+                if (__ballot(list.passes(bm))) {
+                    uint32_t mask = 0;
+#pragma unroll
+                    for (int i = 0; i < NX; ++i)
+                        if (list.passes(xs[i]) && b + (i / VEC) * 256 + tid < v1) mask |= 1u << i;
+                    for (uint64_t todo = __ballot(mask != 0); todo; todo = __ballot(mask != 0)) {
+                        const int slot = __builtin_ctz(mask | 0x80000000u);
+                        mask &= mask - 1;
+                        float v = xs[0];
+#pragma unroll
+                        for (int i = 1; i < NX; ++i) v = slot == i ? xs[i] : v;
+                        list.insert(todo, lp_key(v, head + (b + (slot / VEC) * 256 + tid) * VEC + slot % VEC), p.top_k);
+                    }
                 }
-                const uint64_t who = __ballot(above == p.top_k - 1);
-                lim = who ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, t), __builtin_ctzll(who)))
-                          : -INFINITY;
-            } else if (filled) {
-                strict = true;  // an equal value of a later batch has a higher index
             }
-            if (__ballot(strict ? bm > lim : bm >= lim) == 0) continue;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int v = b + u * 256 + tid;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) offer(xs[u * VEC + j], head + v * VEC + j, v < v1);
-            }
+            for (int u = 0; u < U; ++u) cur[u] = nxt[u];
         }
         if (split == 0 && wave == 0 && head + tail > 0) {       // at most 14 single tokens
             const bool valid = lane < head + tail;
             const int i = lane < head ? lane : head + nvec * VEC + (lane - head);
             float xs[1] = {valid ? to_f32(x[i]) : -INFINITY};
             lp_add<1>(st, xs, xs[0], c);
-            strict = false;
-            if (p.top_k > 0) offer(xs[0], i, valid);
+            if (p.top_k > 0) {
+                list.strict = false;
+                list.insert(__ballot(valid && list.passes(xs[0])), lp_key(xs[0], i), p.top_k);
+            }
         }
         st = lp_across<64>(st, c);
         if (lane == 0) part[wave] = st;
-        if (lane < p.top_k) keys[wave * p.top_k + lane] = list;
+        if (lane < p.top_k) keys[wave * p.top_k + lane] = list.key;
         __syncthreads();
         st = lp_merge(lp_merge(part[0], part[1], c), lp_merge(part[2], part[3], c), c);
         if (p.splits > 1) {
@@ -319,81 +408,96 @@ __global__ __launch_bounds__(256) void logprob_long_kernel(LogprobArgs p) {
             if (tid < p.top_k) p.part_top[unit * p.top_k + tid] = 0;     // (a split may hold fewer than top_k tokens)
             __syncthreads();
             lp_rank(keys, 4 * p.top_k, p.top_k, [&](int k, uint64_t key) { p.part_top[unit * p.top_k + k] = key; });
+        } else if (!lp_ordinary(st, c)) {
+            lp_walk_row<T>(p, row, tok, part, keys);
         } else {
-            if (tid == 0) lp_finish_row<T>(p, row, tok, st);
-            const float ls = lp_log_sum(st);
-            if (p.top_k > 0) {
-                if (lp_not_a_number(st)) lp_walk_top<T>(p, row, st, ls, keys);
-                else lp_rank(keys, 4 * p.top_k, p.top_k, [&](int k, uint64_t key) { lp_put_alternative<T>(p, row, k, key, st, ls); });
-            }
+            const LpRow q(st.m, lp_log2_sum(st), c, false);
+            if (tid == 0) lp_finish_row<T>(p, row, tok, st, q);
+            lp_rank(keys, 4 * p.top_k, p.top_k, [&](int k, uint64_t key) { lp_put_alternative<T>(p, row, k, key, q); });
         }
         __syncthreads();            // part[] and keys[] are reused by the next unit
     }
 }
-// joins the splits of a row
+// Joins the splits of a row.  Of their sorted lists only keys that reach the k-th largest of the lists' first ceil(k /
+// splits) entries can be among the best: mostly k and a few more.
+#define LP_JOIN_KEYS 1024
 template <typename T>
 __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs p) {
-    __shared__ uint64_t keys[1024];
+    __shared__ uint64_t keys[LP_JOIN_KEYS], heads[128], limit;
+    __shared__ LpStat part[4];
+    __shared__ int count;
     const long long row = blockIdx.x;
     const long long tok = lp_token(p, row);
-    const int tid = threadIdx.x, lane = tid & 63, n = p.splits * p.top_k;
+    const int tid = threadIdx.x, lane = tid & 63, k = p.top_k, n = p.splits * k;
     if (tok == p.ignore) {
         if (tid == 0) lp_ignored_row(p, row);
         return;
     }
-    const float c = p.inv_t * LP_LOG2E;
     LpStat st{-INFINITY, 0.f, 0.f};         // (every wave merges all splits: no exchange between waves)
     for (int s = lane; s < p.splits; s += 64) {
         const float* q = p.part_stat + (row * p.splits + s) * 4;
-        st = lp_merge(st, LpStat{q[0], q[1], q[2]}, c);
+        st = lp_merge(st, LpStat{q[0], q[1], q[2]}, p.c);
     }
-    st = lp_across<64>(st, c);
-    const float ls = lp_log_sum(st);
-    if (tid == 0) lp_finish_row<T>(p, row, tok, st);
-    if (p.top_k == 0) return;
-    if (lp_not_a_number(st)) {
-        lp_walk_top<T>(p, row, st, ls, keys);
+    st = lp_across<64>(st, p.c);
+    if (!lp_ordinary(st, p.c)) {
+        lp_walk_row<T>(p, row, tok, part, keys);
         return;
     }
-    for (int i = tid; i < n; i += 256) keys[i] = p.part_top[row * n + i];
+    const LpRow q(st.m, lp_log2_sum(st), p.c, false);
+    if (tid == 0) lp_finish_row<T>(p, row, tok, st, q);
+    if (k == 0) return;
+    const unsigned long long* top = p.part_top + row * n;
+    const int deep = (k + p.splits - 1) / p.splits, nh = deep * p.splits;       // k <= nh < k + splits <= 96
+    if (tid == 0) { count = 0; limit = 0; }
+    if (tid < nh) heads[tid] = top[(tid / deep) * k + tid % deep];
     __syncthreads();
-    lp_rank(keys, n, p.top_k, [&](int k, uint64_t key) { lp_put_alternative<T>(p, row, k, key, st, ls); });
+    lp_rank(heads, nh, k, [&](int r, uint64_t key) { if (r == k - 1) limit = key; });
+    __syncthreads();
+    for (int i = tid; i < n; i += 256) {
+        const uint64_t key = top[i];
+        if (key != 0 && key >= limit) keys[atomicAdd(&count, 1)] = key;     // (any order: lp_rank sorts)
+    }
+    __syncthreads();
+    lp_rank(keys, count, k, [&](int r, uint64_t key) { lp_put_alternative<T>(p, row, r, key, q); });
 }
 
 // ---- gradient ----------------------------------------------------------------------------------------------------------
 // One pass: each logit read once, each gradient written once.
-struct LpGrad { float m, ls, dent, dlp, k0, inv_t; long long tok; bool zero; };
-__device__ __forceinline__ LpGrad lp_grad_of(const LogprobArgs& p, long long row) {
-    LpGrad g;
-    g.tok = lp_token(p, row);
-    g.m = p.stat_m[row];
-    g.ls = p.stat_ls[row];
-    g.zero = g.tok == p.ignore || (g.m == -INFINITY && g.ls == g.ls);       // ignored, or nothing but -inf
-    g.dlp = p.d_lp ? p.d_lp[row] : 0.f;
-    g.dent = p.d_ent ? p.d_ent[row] : 0.f;
-    g.k0 = (p.d_lse ? p.d_lse[row] : 0.f) - g.dlp - g.dent * p.entropy[row];
-    if (g.tok < 0 || g.tok >= p.vocab) g.k0 = __builtin_nanf("");
-    g.inv_t = p.inv_t;
-    return g;
-}
-__device__ __forceinline__ float lp_grad(const LpGrad& g, float x, int i) {
-    const float lp = (x - g.m) * g.inv_t - g.ls, pr = lp_exp2(lp * LP_LOG2E);
-    float d = pr * (g.k0 - g.dent * fmaxf(lp, -1000.f));
-    if (i == g.tok) d += g.dlp;
-    return g.zero ? 0.f : d * g.inv_t;
-}
+struct LpGrad {
+    LpRow q; float dent, dlp, k0, inv_t; long long tok; bool zero;
+    __device__ __forceinline__ LpGrad(const LogprobArgs& p, long long row, bool short_row)
+        : q(p.stat_m[row], p.stat_l2[row], p.c, short_row), tok(lp_token(p, row)) {
+        zero = tok == p.ignore || q.empty;
+        dlp = p.d_lp ? p.d_lp[row] : 0.f;
+        dent = p.d_ent ? p.d_ent[row] : 0.f;
+        k0 = (p.d_lse ? p.d_lse[row] : 0.f) - dlp - dent * p.entropy[row];
+        if (tok < 0 || tok >= p.vocab) k0 = __builtin_nanf("");
+        inv_t = p.inv_t;
+        k0 *= inv_t;
+        dlp *= inv_t;
+        dent *= inv_t * LP_LN2;         // (with log2p below)
+    }
+    template <bool NEAR> __device__ __forceinline__ float of(float x, int i) const {
+        const float lp = (NEAR ? __builtin_fmaf(x, q.c, -q.r) : (x - q.m) * q.c) - q.l2, pr = lp_exp2(lp);
+        const float d = pr * __builtin_fmaf(-dent, fmaxf(lp, -1000.f), k0);
+        return i == tok ? d + dlp : d;
+    }
+    __device__ __forceinline__ float at(float x, int i) const {
+        return zero ? 0.f : q.near ? of<true>(x, i) : of<false>(x, i);
+    }
+};
 template <typename T, int E, int G>
 __global__ __launch_bounds__(256) void logprob_short_bwd_kernel(LogprobArgs p) {
     const int l = threadIdx.x & (G - 1);
     const long long step = (long long)gridDim.x * (256 / G);
     for (long long row = (long long)blockIdx.x * (256 / G) + threadIdx.x / G; row < p.rows; row += step) {
-        const LpGrad g = lp_grad_of(p, row);
+        const LpGrad g(p, row, true);
         const T* x = (const T*)p.logits + row * p.ld;
         T* dx = (T*)p.d_logits + row * p.vocab;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int i = l + e * G;
-            if (i < p.vocab) dx[i] = from_f32<T>(lp_grad(g, g.zero ? 0.f : to_f32(x[i]), i));
+            if (i < p.vocab) dx[i] = from_f32<T>(g.at(g.zero ? 0.f : to_f32(x[i]), i));
         }
     }
 }
@@ -405,7 +509,7 @@ __global__ __launch_bounds__(256) void logprob_long_bwd_kernel(LogprobArgs p, in
     for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const long long row = unit / parts;
         const int part = (int)(unit - row * parts);
-        const LpGrad g = lp_grad_of(p, row);
+        const LpGrad g(p, row, false);
         const T* x = (const T*)p.logits + row * p.ld;
         T* dx = (T*)p.d_logits + row * p.vocab;
         const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), p.vocab);
@@ -423,9 +527,13 @@ __global__ __launch_bounds__(256) void logprob_long_bwd_kernel(LogprobArgs p, in
             const int v = v0 + u * 256 + tid;
             if (v >= nvec) continue;
             vec16<T> o;
+            if (g.zero || !g.q.near) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                o.e[j] = from_f32<T>(lp_grad(g, g.zero ? 0.f : to_f32(q[u].e[j]), head + v * VEC + j));
+                for (int j = 0; j < VEC; ++j) o.e[j] = from_f32<T>(g.zero ? 0.f : g.of<false>(to_f32(q[u].e[j]), head + v * VEC + j));
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) o.e[j] = from_f32<T>(g.of<true>(to_f32(q[u].e[j]), head + v * VEC + j));
+            }
             T* to = dx + head + (long long)v * VEC;
             if (wide) {
                 *reinterpret_cast<vec16<T>*>(to) = o;
@@ -436,7 +544,7 @@ __global__ __launch_bounds__(256) void logprob_long_bwd_kernel(LogprobArgs p, in
         }
         if (part == 0 && tid < head + tail) {
             const int i = tid < head ? tid : head + nvec * VEC + (tid - head);
-            dx[i] = from_f32<T>(lp_grad(g, g.zero ? 0.f : to_f32(x[i]), i));
+            dx[i] = from_f32<T>(g.at(g.zero ? 0.f : to_f32(x[i]), i));
         }
     }
 }
@@ -453,7 +561,7 @@ static int lp_splits(long long rows, int vocab, int top_k) {
     long long s = (1024 + rows - 1) / rows;
     if (s > vocab / 4096) s = vocab / 4096;
     if (s > 64) s = 64;
-    if (top_k > 0 && s > 1024 / top_k) s = 1024 / top_k;
+    if (top_k > 0 && s > LP_JOIN_KEYS / top_k) s = LP_JOIN_KEYS / top_k;
     return s < 2 ? 1 : (int)s;
 }
 PDA_EXPORT int pda_logprob_splits(long long rows, int vocab, int top_k) { return lp_splits(rows, vocab, top_k); }

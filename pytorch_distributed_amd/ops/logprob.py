@@ -16,13 +16,14 @@ from ._seq import TYPE_CODES, check_floating, check_int, launched, native, on_de
 MAX_TOP = 32        # csrc/logprob.hip LP_MAX_TOP
 TokenLogprobs = namedtuple("TokenLogprobs", "logprob, entropy, logsumexp, top_logprobs, top_tokens")
 
+_LOG2E = 1.4426950408889634
 _vp, _i64 = ctypes.c_void_p, ctypes.c_longlong
 
 
 class _Args(ctypes.Structure):      # mirrors LogprobArgs in csrc/logprob.hip
     _fields_ = [("logits", _vp), ("ld", _i64), ("rows", _i64), ("vocab", ctypes.c_int), ("tokens", _vp),
-                ("tok64", ctypes.c_int), ("ignore", _i64), ("inv_t", ctypes.c_float), ("top_k", ctypes.c_int),
-                ("logprob", _vp), ("entropy", _vp), ("lse", _vp), ("stat_m", _vp), ("stat_ls", _vp), ("top_lp", _vp),
+                ("tok64", ctypes.c_int), ("ignore", _i64), ("inv_t", ctypes.c_float), ("c", ctypes.c_float), ("top_k", ctypes.c_int),
+                ("logprob", _vp), ("entropy", _vp), ("lse", _vp), ("stat_m", _vp), ("stat_l2", _vp), ("top_lp", _vp),
                 ("top_id", _vp), ("d_lp", _vp), ("d_ent", _vp), ("d_lse", _vp), ("d_logits", _vp),
                 ("splits", ctypes.c_int), ("part_stat", _vp), ("part_top", _vp)]
 
@@ -70,6 +71,7 @@ def _backward_torch(x, tokens, m, ls, ent, d_lp, d_ent, d_lse, inv_t, ignore):
 def _fill(args, x, tokens, inv_t, ignore):
     args.logits, args.ld, args.rows, args.vocab = ptr(x), x.stride(0), x.shape[0], x.shape[1]
     args.tokens, args.tok64, args.ignore, args.inv_t = ptr(tokens), int(tokens.dtype == torch.int64), ignore, inv_t
+    args.c = inv_t * _LOG2E
     return args
 
 
@@ -85,7 +87,7 @@ class _TokenLogprobs(torch.autograd.Function):
             top = torch.empty(n, top_k, dtype=torch.float32, device=x.device)
             ids = torch.empty(n, top_k, dtype=torch.int64, device=x.device)
             args = _fill(_Args(), x, tokens, inv_t, ignore)
-            args.logprob, args.entropy, args.lse, args.stat_m, args.stat_ls = map(ptr, (lp, ent, lse, m, ls))
+            args.logprob, args.entropy, args.lse, args.stat_m, args.stat_l2 = map(ptr, (lp, ent, lse, m, ls))
             args.top_lp, args.top_id, args.top_k = ptr(top), ptr(ids), top_k
             args.splits = native("pda_logprob_splits")(_i64(n), x.shape[1], top_k)
             if args.splits > 1:     # long rows in parts, joined by a second launch
@@ -113,7 +115,7 @@ class _TokenLogprobs(torch.autograd.Function):
         d_lp, d_ent, d_lse = (None if t is None else t.contiguous() for t in (d_lp, d_ent, d_lse))
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         args = _fill(_Args(), x, tokens, inv_t, ignore)
-        args.entropy, args.stat_m, args.stat_ls = map(ptr, (ent, m, ls))
+        args.entropy, args.stat_m, args.stat_l2 = map(ptr, (ent, m, ls))
         args.d_lp, args.d_ent, args.d_lse, args.d_logits = map(ptr, (d_lp, d_ent, d_lse, dx))
         with on_device(x):
             launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "token_logprobs backward")
