@@ -318,9 +318,9 @@ struct LpList {
 // sorted over its lanes.  A value is looked at again only if it passes the wave's k-th best, which the first batch sets to
 // the k-th largest of the lanes' maxima; a wave of n values then inserts about k (2 + ln(n / 2048)) of them, each by a
 // ballot and a shift by one lane.
-template <typename T>
-__global__ __launch_bounds__(256) void logprob_long_kernel(LogprobArgs p) {
-    constexpr int VEC = 16 / sizeof(T), U = 4, NX = U * VEC;
+template <typename T, bool TOP>
+__global__ __launch_bounds__(256, 4) void logprob_long_kernel(LogprobArgs p) {
+    constexpr int VEC = 16 / sizeof(T), U = 2, NX = U * VEC;
     __shared__ LpStat part[4];
     __shared__ uint64_t keys[4 * LP_MAX_TOP];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -342,55 +342,60 @@ __global__ __launch_bounds__(256) void logprob_long_kernel(LogprobArgs p) {
         const vec16<T>* xv = reinterpret_cast<const vec16<T>*>(x + head);
         LpStat st{-INFINITY, 0.f, 0.f};
         LpList list;
-        vec16<T> cur[U], nxt[U];
+        auto fetch = [&](vec16<T> (&raw)[U], int b) {
+            if (b + U * 256 <= v1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int v = v0 + u * 256 + tid;
-            if (v < v1) cur[u] = xv[v];
-        }
-        for (int b = v0; b < v1; b += 256 * U) {
+                for (int u = 0; u < U; ++u) raw[u] = xv[b + u * 256 + tid];
+            } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int v = b + (U + u) * 256 + tid;
-                if (v < v1) nxt[u] = xv[v];
-            }
-            float xs[NX], bm = -INFINITY;
+                for (int u = 0; u < U; ++u) {
+                    const int v = b + u * 256 + tid;
+                    if (v < v1) {
+                        raw[u] = xv[v];
+                    } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const bool in = b + u * 256 + tid < v1;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) xs[u * VEC + j] = in ? to_f32(cur[u].e[j]) : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < NX; ++i) bm = fmaxf(bm, xs[i]);
-            lp_add<NX>(st, xs, bm, c);
-            if (p.top_k > 0) {
-                if (b == v0) list.first_limit(bm, p.top_k);
-                else if (list.full) list.strict = true;     // an equal value of a later batch has a higher index
-                if (__ballot(list.passes(bm))) {
-                    uint32_t mask = 0;
-#pragma unroll
-                    for (int i = 0; i < NX; ++i)
-                        if (list.passes(xs[i]) && b + (i / VEC) * 256 + tid < v1) mask |= 1u << i;
-                    for (uint64_t todo = __ballot(mask != 0); todo; todo = __ballot(mask != 0)) {
-                        const int slot = __builtin_ctz(mask | 0x80000000u);
-                        mask &= mask - 1;
-                        float v = xs[0];
-#pragma unroll
-                        for (int i = 1; i < NX; ++i) v = slot == i ? xs[i] : v;
-                        list.insert(todo, lp_key(v, head + (b + (slot / VEC) * 256 + tid) * VEC + slot % VEC), p.top_k);
+                        for (int j = 0; j < VEC; ++j) raw[u].e[j] = from_f32<T>(-INFINITY);
                     }
                 }
             }
+        };
+        auto take = [&](const vec16<T> (&raw)[U], int b) {
+            float xs[NX], bm = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < U; ++u) cur[u] = nxt[u];
+            for (int i = 0; i < NX; ++i) { xs[i] = to_f32(raw[i / VEC].e[i % VEC]); bm = fmaxf(bm, xs[i]); }
+            lp_add<NX>(st, xs, bm, c);
+            if (!TOP) return;
+            if (b == v0) list.first_limit(bm, p.top_k);
+            else if (list.full) list.strict = true;         // an equal value of a later batch has a higher index
+            if (__ballot(list.passes(bm)) == 0) return;
+            uint32_t mask = 0;
+#pragma unroll
+            for (int i = 0; i < NX; ++i)
+                if (list.passes(xs[i]) && b + (i / VEC) * 256 + tid < v1) mask |= 1u << i;
+            for (uint64_t todo = __ballot(mask != 0); todo; todo = __ballot(mask != 0)) {
+                const int slot = __builtin_ctz(mask | 0x80000000u);
+                mask &= mask - 1;
+                float v = xs[0];
+#pragma unroll
+                for (int i = 1; i < NX; ++i) v = slot == i ? xs[i] : v;
+                list.insert(todo, lp_key(v, head + (b + (slot / VEC) * 256 + tid) * VEC + slot % VEC), p.top_k);
+            }
+        };
+        vec16<T> even[U], odd[U];
+        fetch(even, v0);
+        for (int b = v0; b < v1; b += 2 * 256 * U) {
+            fetch(odd, b + 256 * U);
+            take(even, b);
+            if (b + 256 * U >= v1) break;
+            fetch(even, b + 2 * 256 * U);
+            take(odd, b + 256 * U);
         }
         if (split == 0 && wave == 0 && head + tail > 0) {       // at most 14 single tokens
             const bool valid = lane < head + tail;
             const int i = lane < head ? lane : head + nvec * VEC + (lane - head);
             float xs[1] = {valid ? to_f32(x[i]) : -INFINITY};
             lp_add<1>(st, xs, xs[0], c);
-            if (p.top_k > 0) {
+            if (TOP) {
                 list.strict = false;
                 list.insert(__ballot(valid && list.passes(xs[0])), lp_key(xs[0], i), p.top_k);
             }
@@ -477,13 +482,15 @@ struct LpGrad {
         dlp *= inv_t;
         dent *= inv_t * LP_LN2;         // (with log2p below)
     }
-    template <bool NEAR> __device__ __forceinline__ float of(float x, int i) const {
-        const float lp = (NEAR ? __builtin_fmaf(x, q.c, -q.r) : (x - q.m) * q.c) - q.l2, pr = lp_exp2(lp);
-        const float d = pr * __builtin_fmaf(-dent, fmaxf(lp, -1000.f), k0);
-        return i == tok ? d + dlp : d;
+    // without the taken token's own dlp
+    template <bool NEAR> __device__ __forceinline__ float of(float x) const {
+        const float lp = (NEAR ? __builtin_fmaf(x, q.c, -q.r) : (x - q.m) * q.c) - q.l2;
+        return lp_exp2(lp) * __builtin_fmaf(-dent, fmaxf(lp, -1000.f), k0);
     }
     __device__ __forceinline__ float at(float x, int i) const {
-        return zero ? 0.f : q.near ? of<true>(x, i) : of<false>(x, i);
+        if (zero) return 0.f;
+        const float d = q.near ? of<true>(x) : of<false>(x);
+        return i == tok ? d + dlp : d;
     }
 };
 template <typename T, int E, int G>
@@ -501,9 +508,10 @@ __global__ __launch_bounds__(256) void logprob_short_bwd_kernel(LogprobArgs p) {
         }
     }
 }
-template <typename T>
+#define LP_BWD_U 4      // 16-byte loads in flight per thread: 2 / 4 / 8 took 111 / 107 / 115 us at 4096 x 32000 bf16
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void logprob_long_bwd_kernel(LogprobArgs p, int parts) {
-    constexpr int VEC = 16 / sizeof(T), U = 4;
+    constexpr int VEC = 16 / sizeof(T), U = LP_BWD_U;
     const int tid = threadIdx.x;
     const long long units = p.rows * parts;
     for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
@@ -515,28 +523,38 @@ __global__ __launch_bounds__(256) void logprob_long_bwd_kernel(LogprobArgs p, in
         const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), p.vocab);
         const int nvec = (p.vocab - head) / VEC, tail = (p.vocab - head) - nvec * VEC;
         const bool wide = (reinterpret_cast<uintptr_t>(dx + head) & 15) == 0;      // both on the 16-byte grid together
-        const int v0 = part * (256 * U);
+        const int taken = g.zero ? -1 : (int)min(max(g.tok, -1ll), (long long)p.vocab) - head;  // counted from the first vector
+        const int v0 = part * (256 * U) + tid;
         vec16<T> q[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int v = v0 + u * 256 + tid;
-            if (v < nvec && !g.zero) q[u] = *reinterpret_cast<const vec16<T>*>(x + head + (long long)v * VEC);
+            if (v0 + u * 256 < nvec && !g.zero) q[u] = *reinterpret_cast<const vec16<T>*>(x + head + (long long)(v0 + u * 256) * VEC);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int v = v0 + u * 256 + tid;
+            const int v = v0 + u * 256;
             if (v >= nvec) continue;
-            vec16<T> o;
-            if (g.zero || !g.q.near) {
+            float d[VEC];
+            if (g.zero) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) o.e[j] = from_f32<T>(g.zero ? 0.f : g.of<false>(to_f32(q[u].e[j]), head + v * VEC + j));
+                for (int j = 0; j < VEC; ++j) d[j] = 0.f;
+            } else if (g.q.near) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) d[j] = g.of<true>(to_f32(q[u].e[j]));
             } else {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) o.e[j] = from_f32<T>(g.of<true>(to_f32(q[u].e[j]), head + v * VEC + j));
+                for (int j = 0; j < VEC; ++j) d[j] = g.of<false>(to_f32(q[u].e[j]));
             }
+            if (taken >= v * VEC && taken < v * VEC + VEC) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) d[j] += taken - v * VEC == j ? g.dlp : 0.f;
+            }
+            vec16<T> o;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) o.e[j] = from_f32<T>(d[j]);
             T* to = dx + head + (long long)v * VEC;
             if (wide) {
-                *reinterpret_cast<vec16<T>*>(to) = o;
+                store16<STREAM>(to, o);
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) to[j] = o.e[j];
@@ -580,14 +598,18 @@ static void lp_launch(const LogprobArgs& p, bool backward, hipStream_t stream) {
     else if (p.vocab <= 256) lp_launch_short<T, 4, 64>(p, backward, stream);
     else if (p.vocab <= LP_SHORT) lp_launch_short<T, 16, 64>(p, backward, stream);
     else if (backward) {
-        constexpr int PART = 256 * 4 * (16 / sizeof(T));
+        constexpr int PART = 256 * LP_BWD_U * (16 / sizeof(T));
         const int parts = (p.vocab + PART - 1) / PART;
         const long long units = p.rows * parts;
-        hipLaunchKernelGGL(logprob_long_bwd_kernel<T>, dim3((unsigned)(units < 1048576 ? units : 1048576)), dim3(256), 0,
-                           stream, p, parts);
+        const dim3 grid((unsigned)(units < 1048576 ? units : 1048576)), block(256);
+        if (seq_streams(p.rows * p.vocab * (long long)sizeof(T)))
+            hipLaunchKernelGGL((logprob_long_bwd_kernel<T, true>), grid, block, 0, stream, p, parts);
+        else hipLaunchKernelGGL((logprob_long_bwd_kernel<T, false>), grid, block, 0, stream, p, parts);
     } else {
         const long long units = p.rows * p.splits;
-        hipLaunchKernelGGL(logprob_long_kernel<T>, dim3((unsigned)(units < 1048576 ? units : 1048576)), dim3(256), 0, stream, p);
+        const dim3 grid((unsigned)(units < 1048576 ? units : 1048576)), block(256);
+        if (p.top_k > 0) hipLaunchKernelGGL((logprob_long_kernel<T, true>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((logprob_long_kernel<T, false>), grid, block, 0, stream, p);
         if (p.splits > 1) hipLaunchKernelGGL(logprob_join_kernel<T>, dim3((unsigned)p.rows), dim3(256), 0, stream, p);
     }
 }

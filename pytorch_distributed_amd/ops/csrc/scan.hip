@@ -16,24 +16,28 @@ struct ScanArgs {
     const float* h0; const float* dlast;    // [B][D], may be null
     const void* lengths; int len64;         // [B] or null: steps from the length on are no part of a sequence
     void* h; float* last;                   // [B][T][D] contiguous, [B][D]
-    float* carry;                           // [B][tiles][D]: the state in front of every tile (null: no backward pass)
+    float* carry;                           // [B][carries][D]: the state in front of every carry_len steps (null: not kept)
     float* sums;                            // [B][chunks][2][D]: the chunks' partial recurrences (chunks > 1)
     void* dx; void* dg; float* dh0;
     int B, T, D, logit, mix, reverse;
-    int chunks;                             // ScanPlan
+    int chunks, chunk_len, carry_len, carries;      // ScanPlan
 };
 
-struct Gate { float a, c; };                // a and c = 1 - a
-__device__ __forceinline__ Gate gate_of(float g, int logit) {
-    if (!logit) return Gate{g, 1.f - g};
-    const float e = __expf(-fabsf(g)), r = 1.f / (1.f + e);     // sigmoid(|g|); the other side is e r
-    return g >= 0.f ? Gate{r, e * r} : Gate{e * r, r};
+// k = a where a <= 1/2, else -c (its sign says which); c = 1 - a.  For decay gates k = a.
+struct Gate { float k, c; };
+template <bool LOGIT>
+__device__ __forceinline__ Gate gate_of(float g) {
+    if (!LOGIT) return Gate{g, 1.f - g};
+    const float e = __builtin_amdgcn_exp2f(g * 1.44269504088896341f), c = __builtin_amdgcn_rcpf(1.f + e);     // a = e c
+    return Gate{c <= 0.5f ? -c : e * c, c};
 }
-__device__ __forceinline__ float decayed(float h, Gate g, int logit) {      // a h
-    return logit && g.c <= 0.5f ? __builtin_fmaf(-g.c, h, h) : g.a * h;
+template <bool LOGIT>
+__device__ __forceinline__ float decayed(float h, Gate g) {         // a h
+    return LOGIT ? __builtin_fmaf(g.k, h, __builtin_bit_cast(int, g.k) < 0 ? h : 0.f) : g.k * h;
 }
-__device__ __forceinline__ float scan_step(float h, float x, Gate g, int logit, int mix) {
-    return decayed(h, g, logit) + (mix ? g.c * x : x);
+template <bool LOGIT, bool MIX>
+__device__ __forceinline__ float scan_step(float h, float x, Gate g) {
+    return MIX ? __builtin_fmaf(g.c, x, decayed<LOGIT>(h, g)) : decayed<LOGIT>(h, g) + x;
 }
 __device__ __forceinline__ int scan_length(const ScanArgs& p, int b) {
     if (p.lengths == nullptr) return p.T;
@@ -55,16 +59,48 @@ __device__ __forceinline__ int scan_length(const ScanArgs& p, int b) {
 // Where the slabs do not fill the card, the steps are cut into chunks: scan_sum_kernel leaves every chunk's product of
 // gates and end state, and each chunk's workgroup folds those in front of it before it starts.  x and gate are then read
 // twice.
-template <typename T> struct ScanShape { static constexpr int VEC = 16 / sizeof(T), CL = 4, L = 32 / VEC, NT = 256; };
+#ifndef SC_FL
+#define SC_FNT 512
+#define SC_FL 4
+#define SC_BNT 256
+#define SC_BL 4
+#endif
+#ifndef SCAN_CL
+#define SCAN_CL 8
+#endif
+#ifndef SC_TARGET
+#define SC_TARGET 256
+#endif
+// a forward tile holds a whole number of backward tiles: the forward pass leaves the state in front of each of those
+template <typename T> struct ScanFwd { static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = SC_FL * 8 / VEC, NT = SC_FNT; };
+template <typename T> struct ScanBwd { static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = SC_BL * 8 / VEC, NT = SC_BNT; };
 struct ScanRow { static constexpr int VEC = 1, CL = 1, L = 8, NT = 1024; };     // few channels: one per workgroup
+// The lanes of a wave: SW consecutive ones hold consecutive runs of steps of one group of VEC channels, so that a scan
+// over steps moves along a DPP row.
+template <typename S> struct ScanLane {
+    static constexpr int SW = 64 / S::CL, W = S::CL * S::VEC;
+    int cl, sub;
+    __device__ __forceinline__ ScanLane() : cl(((int)threadIdx.x & 63) / SW), sub((int)(threadIdx.x >> 6) * SW + ((int)threadIdx.x & (SW - 1))) {}
+};
+
+// How a kernel touches memory: element by element (any strides), in 16-byte accesses (contiguous channels on the 16-byte
+// grid), or so with stores past the caches.
+#define SCAN_ANY 0
+#define SCAN_WIDE 1
+#define SCAN_STREAM 2
 
 struct ScanWhere { int b, chunk, ch0, nch, n; };
 template <typename S>
 __device__ __forceinline__ ScanWhere scan_where(const ScanArgs& p) {
     const int nslab = (p.D + S::CL * S::VEC - 1) / (S::CL * S::VEC);
     ScanWhere w;
-    const int rest = (int)blockIdx.x / nslab;
-    w.ch0 = (((int)blockIdx.x - rest * nslab) * S::CL + (int)threadIdx.x % S::CL) * S::VEC;
+#ifdef SC_XCD
+    const int n8 = (int)gridDim.x / 8, id = (int)blockIdx.x < n8 * 8 ? ((int)blockIdx.x & 7) * n8 + ((int)blockIdx.x >> 3) : (int)blockIdx.x;
+#else
+    const int id = blockIdx.x;
+#endif
+    const int rest = id / nslab;
+    w.ch0 = ((id - rest * nslab) * S::CL + ScanLane<S>().cl) * S::VEC;
     w.nch = min(max(p.D - w.ch0, 0), S::VEC);
     w.b = rest / p.chunks;
     w.chunk = rest - w.b * p.chunks;
@@ -72,86 +108,133 @@ __device__ __forceinline__ ScanWhere scan_where(const ScanArgs& p) {
     return w;
 }
 
-template <typename T, int VEC> struct Raw { T e[VEC]; };
+// VEC elements in whole registers (16-bit ones in pairs)
+template <typename T, int VEC> struct Raw {
+    static constexpr int PER = VEC == 1 ? 1 : 4 / (int)sizeof(T), NW = VEC / PER;
+    uint32_t w[NW];
+    __device__ __forceinline__ void put(int i, T v) {
+        const uint32_t bits = bits_of(v);
+        w[i / PER] = i % PER == 0 ? bits : (w[i / PER] | bits << 16);
+    }
+    __device__ __forceinline__ float get(int i) const { return value_of<T>(w[i / PER], i % PER); }
+};
 // VEC channels at `row`: one 16-byte access where the layout allows it, else element by element
-template <typename T, int VEC>
-__device__ __forceinline__ Raw<T, VEC> scan_load(const T* row, long long cs, bool wide, int nch) {
+template <typename T, int VEC, bool WIDE>
+__device__ __forceinline__ Raw<T, VEC> scan_load(const T* row, long long cs, int nch) {
     Raw<T, VEC> r;
-    if (VEC * sizeof(T) == 16 && wide) {
-        const vec16<T> v = *reinterpret_cast<const vec16<T>*>(row);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) r.e[i] = v.e[i];
+    if constexpr (WIDE) {
+        const uint4 v = *reinterpret_cast<const uint4*>(row);
+        r.w[0] = v.x;
+        r.w[1] = v.y;
+        r.w[2] = v.z;
+        r.w[3] = v.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) r.e[i] = i < nch ? row[i * cs] : from_f32<T>(0.f);
+        for (int i = 0; i < VEC; ++i) r.put(i, i < nch ? row[i * cs] : from_f32<T>(0.f));
     }
     return r;
 }
-template <typename T, int VEC>
-__device__ __forceinline__ void scan_store(T* row, const float (&v)[VEC], bool wide, int nch) {
-    if (VEC * sizeof(T) == 16 && wide) {
+template <typename T, int VEC, int MODE>
+__device__ __forceinline__ void scan_store(T* row, const float (&v)[VEC], int nch) {
+    if constexpr (MODE != SCAN_ANY) {
         vec16<T> o;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o.e[i] = from_f32<T>(v[i]);
-        *reinterpret_cast<vec16<T>*>(row) = o;
+        store16<MODE == SCAN_STREAM>(row, o);
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
             if (i < nch) row[i] = from_f32<T>(v[i]);
     }
 }
-template <typename T, int VEC>
-__device__ __forceinline__ bool scan_wide(const void* base, const long long (&s)[3], int D) {
-    return VEC * sizeof(T) == 16 && s[2] == 1 && D % VEC == 0 && s[0] % VEC == 0 && s[1] % VEC == 0 &&
-           (reinterpret_cast<uintptr_t>(base) & 15) == 0;
-}
-
 // joins a later part (a, h) behind an earlier one (pa, ph): state -> a (pa state + ph) + h
 #define SCAN_JOIN(a, h, pa, ph) do { h = __builtin_fmaf(a, ph, h); a *= pa; } while (0)
 
 // Exclusive scan of the threads' parts over the workgroup, in step order (UP) or against it, applied to the state `in` in
 // front of the tile: -> the state in front of this thread's steps; `in` becomes the state behind the tile.
 // part: [waves][CL * VEC] in LDS; the caller separates two uses of one buffer by a barrier.
+template <int O, bool UP, int BANKS = 0xf>
+__device__ __forceinline__ float dpp_shift(float none, float v) {       // lane i of a row of 16 gets lane i -+ O's, or `none`
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
+                                                                 (UP ? 0x110 : 0x100) + O, 0xf, BANKS, false));
+}
+template <int O, int SW, bool UP>
+__device__ __forceinline__ void scan_lanes_step(float& A, float& H) {
+    if constexpr (O < SW) {
+        const int i = threadIdx.x & (SW - 1);
+        const bool on = UP ? i >= O : i < SW - O;
+        float pa, ph;
+        if constexpr (O < 16) {
+            constexpr int BANKS = SW == 8 && O == 4 ? (UP ? 0xa : 0x5) : 0xf;      // (the lanes of a group that have a partner)
+            pa = dpp_shift<O, UP, BANKS>(1.f, A);
+            ph = dpp_shift<O, UP, BANKS>(0.f, H);
+            if (SW < 16 && BANKS == 0xf) { pa = on ? pa : 1.f; ph = on ? ph : 0.f; }
+        } else {
+            pa = UP ? __shfl_up(A, O, 64) : __shfl_down(A, O, 64);
+            ph = UP ? __shfl_up(H, O, 64) : __shfl_down(H, O, 64);
+            pa = on ? pa : 1.f;
+            ph = on ? ph : 0.f;
+        }
+        if constexpr (SW > 16 && O < 16) {      // rows of 16 are joined by the steps of 16 and 32: a wave's lanes in order
+            const int r = threadIdx.x & 15;
+            const float qa = UP ? __shfl_up(A, O, 64) : __shfl_down(A, O, 64), qh = UP ? __shfl_up(H, O, 64) : __shfl_down(H, O, 64);
+            const bool over = UP ? r < O : r >= 16 - O;
+            pa = over && on ? qa : pa;
+            ph = over && on ? qh : ph;
+        }
+        SCAN_JOIN(A, H, pa, ph);
+    }
+}
+// inclusive over the SW lanes of a channel group
+template <int SW, bool UP>
+__device__ __forceinline__ void scan_lanes(float& A, float& H) {
+    scan_lanes_step<1, SW, UP>(A, H);
+    scan_lanes_step<2, SW, UP>(A, H);
+    scan_lanes_step<4, SW, UP>(A, H);
+    scan_lanes_step<8, SW, UP>(A, H);
+    scan_lanes_step<16, SW, UP>(A, H);
+    scan_lanes_step<32, SW, UP>(A, H);
+}
 template <typename S, bool UP>
 __device__ __forceinline__ void scan_across(float (&A)[S::VEC], float (&H)[S::VEC], float (&in)[S::VEC], float2* part) {
-    constexpr int NW = S::NT / 64, W = S::CL * S::VEC;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cl = threadIdx.x % S::CL;
+    constexpr int NW = S::NT / 64, W = S::CL * S::VEC, SW = ScanLane<S>::SW;
+    const int wave = threadIdx.x >> 6, cl = ScanLane<S>().cl, i = threadIdx.x & (SW - 1);
 #pragma unroll
-    for (int o = S::CL; o < 64; o <<= 1) {
-        const bool on = UP ? lane >= o : lane < 64 - o;
-#pragma unroll
-        for (int v = 0; v < S::VEC; ++v) {
-            const float pa = UP ? __shfl_up(A[v], o, 64) : __shfl_down(A[v], o, 64);
-            const float ph = UP ? __shfl_up(H[v], o, 64) : __shfl_down(H[v], o, 64);
-            if (on) SCAN_JOIN(A[v], H[v], pa, ph);
-        }
-    }
-    const bool end = UP ? lane >= 64 - S::CL : lane < S::CL;
-    if (end) {
+    for (int v = 0; v < S::VEC; ++v) scan_lanes<SW, UP>(A[v], H[v]);
+    if (i == (UP ? SW - 1 : 0)) {
 #pragma unroll
         for (int v = 0; v < S::VEC; ++v) part[wave * W + cl * S::VEC + v] = make_float2(A[v], H[v]);
     }
-    const bool first = UP ? lane < S::CL : lane >= 64 - S::CL;
+    const bool first = i == (UP ? 0 : SW - 1);
 #pragma unroll
-    for (int v = 0; v < S::VEC; ++v) {
-        const float pa = UP ? __shfl_up(A[v], S::CL, 64) : __shfl_down(A[v], S::CL, 64);
-        const float ph = UP ? __shfl_up(H[v], S::CL, 64) : __shfl_down(H[v], S::CL, 64);
+    for (int v = 0; v < S::VEC; ++v) {      // exclusive: the neighbour's
+        float pa, ph;
+        if constexpr (SW <= 16) {
+            pa = dpp_shift<1, UP>(1.f, A[v]);
+            ph = dpp_shift<1, UP>(0.f, H[v]);
+        } else {
+            pa = UP ? __shfl_up(A[v], 1, 64) : __shfl_down(A[v], 1, 64);
+            ph = UP ? __shfl_up(H[v], 1, 64) : __shfl_down(H[v], 1, 64);
+        }
         A[v] = first ? 1.f : pa;
         H[v] = first ? 0.f : ph;
     }
     __syncthreads();
+    float mine[S::VEC];
 #pragma unroll
-    for (int v = 0; v < S::VEC; ++v) {
-        float mine = in[v];
+    for (int v = 0; v < S::VEC; ++v) mine[v] = in[v];
+#pragma unroll 2
+    for (int k = 0; k < NW; ++k) {          // (not unrolled further: the parts of all waves at once would take 2 VEC NW registers)
+        const int w = UP ? k : NW - 1 - k;
 #pragma unroll
-        for (int k = 0; k < NW; ++k) {
-            const int w = UP ? k : NW - 1 - k;
-            if (w == wave) mine = in[v];
+        for (int v = 0; v < S::VEC; ++v) {
             const float2 t = part[w * W + cl * S::VEC + v];
+            if (w == wave) mine[v] = in[v];
             in[v] = __builtin_fmaf(t.x, in[v], t.y);
         }
-        H[v] = __builtin_fmaf(A[v], mine, H[v]);
     }
+#pragma unroll
+    for (int v = 0; v < S::VEC; ++v) H[v] = __builtin_fmaf(A[v], mine[v], H[v]);
 }
 
 // the state in front of this workgroup's chunk: `in` carried over the chunks before it (UP) or behind it
@@ -169,69 +252,97 @@ __device__ __forceinline__ void scan_fold_chunks(const ScanArgs& p, const ScanWh
 // tiles [first, last) of a chunk
 template <typename S> struct ScanTiles {
     static constexpr int SUB = S::NT / S::CL, TILE = SUB * S::L;
-    int tiles, per, first, last;
+    int first, last;
     __device__ __forceinline__ ScanTiles(const ScanArgs& p, int chunk) {
-        tiles = (p.T + TILE - 1) / TILE;
-        per = (tiles + p.chunks - 1) / p.chunks;
-        first = min(chunk * per, tiles);
-        last = min(first + per, tiles);
+        const int begin = min(chunk * p.chunk_len, p.T), end = min(begin + p.chunk_len, p.T);      // chunk_len: whole tiles
+        first = begin / TILE;
+        last = (end + TILE - 1) / TILE;
+        if (begin >= end) last = first;
     }
 };
 
-template <typename T, typename S, bool LOGIT>
+// What a step that does not exist reads: it leaves the state as it is (a = 1, u = 0).
+template <typename T, int VEC, bool LOGIT>
+__device__ __forceinline__ Raw<T, VEC> scan_no_gate() {
+    Raw<T, VEC> r;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) r.put(v, from_f32<T>(LOGIT ? INFINITY : 1.f));
+    return r;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ Raw<T, VEC> scan_nothing() {
+    Raw<T, VEC> r;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) r.put(v, from_f32<T>(0.f));
+    return r;
+}
+
+template <typename T, typename S, bool LOGIT, bool MIX, int MODE>
 __global__ __launch_bounds__(S::NT) void scan_fwd_kernel(ScanArgs p) {
     constexpr int VEC = S::VEC, L = S::L, TILE = ScanTiles<S>::TILE;
     __shared__ float2 part[2][S::NT / 64 * S::CL * VEC];
     const ScanWhere w = scan_where<S>(p);
     const ScanTiles<S> tl(p, w.chunk);
-    const int sub = threadIdx.x / S::CL;
-    const bool xw = scan_wide<T, VEC>(p.x, p.xs, p.D), gw = scan_wide<T, VEC>(p.gate, p.gs, p.D), ow = p.D % VEC == 0;
+    const int sub = ScanLane<S>().sub;
     const T* x = (const T*)p.x + w.b * p.xs[0] + w.ch0 * p.xs[2];
     const T* g = (const T*)p.gate + w.b * p.gs[0] + w.ch0 * p.gs[2];
     T* out = (T*)p.h + (long long)w.b * p.T * p.D + w.ch0;
+    Raw<T, VEC> xr[L], gr[L];
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+            const int i = tile * TILE + sub * L + l;
+            if (i < w.n && w.nch > 0) {
+                const long long t = p.reverse ? w.n - 1 - i : i;
+                xr[l] = scan_load<T, VEC, MODE != SCAN_ANY>(x + t * p.xs[1], p.xs[2], w.nch);
+                gr[l] = scan_load<T, VEC, MODE != SCAN_ANY>(g + t * p.gs[1], p.gs[2], w.nch);
+            } else {
+                xr[l] = scan_nothing<T, VEC>();
+                gr[l] = scan_no_gate<T, VEC, LOGIT>();
+            }
+        }
+    };
+    fetch(tl.first);
     float in[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) in[v] = p.h0 && v < w.nch ? p.h0[(long long)w.b * p.D + w.ch0 + v] : 0.f;
     scan_fold_chunks<S, true>(p, w, in);
     for (int tile = tl.first; tile < tl.last; ++tile) {
         const int i0 = tile * TILE + sub * L;
-        if (p.carry != nullptr && sub == 0) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                if (v < w.nch) p.carry[((long long)w.b * tl.tiles + tile) * p.D + w.ch0 + v] = in[v];
-        }
         float A[L][VEC], H[L][VEC];
-        if (tile * TILE < w.n) {
-            Raw<T, VEC> xr[L], gr[L];
+        float start[VEC];       // the state in front of this thread's steps
 #pragma unroll
-            for (int l = 0; l < L; ++l) {
-                const int i = min(i0 + l, w.n - 1);
-                const long long t = p.reverse ? w.n - 1 - i : i;
-                xr[l] = scan_load<T, VEC>(x + t * p.xs[1], p.xs[2], xw && w.nch > 0, w.nch);
-                gr[l] = scan_load<T, VEC>(g + t * p.gs[1], p.gs[2], gw && w.nch > 0, w.nch);
-            }
+        for (int v = 0; v < VEC; ++v) start[v] = 0.f;
+        if (tile * TILE < w.n) {
             float a[VEC], h[VEC];
 #pragma unroll
             for (int v = 0; v < VEC; ++v) { a[v] = 1.f; h[v] = 0.f; }
 #pragma unroll
             for (int l = 0; l < L; ++l) {
-                const bool on = i0 + l < w.n;
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    const Gate ga = gate_of(to_f32(gr[l].e[v]), LOGIT);
-                    const float hv = scan_step(h[v], to_f32(xr[l].e[v]), ga, LOGIT, p.mix), av = decayed(a[v], ga, LOGIT);
-                    h[v] = on ? hv : h[v];
-                    a[v] = on ? av : a[v];
+                    const Gate ga = gate_of<LOGIT>(gr[l].get(v));
+                    h[v] = scan_step<LOGIT, MIX>(h[v], xr[l].get(v), ga);
+                    a[v] = decayed<LOGIT>(a[v], ga);
                     A[l][v] = a[v];
                     H[l][v] = h[v];
                 }
             }
+            if (tile + 1 < tl.last) fetch(tile + 1);            // in flight over the scan and the stores
             scan_across<S, true>(a, h, in, part[tile & 1]);     // (two buffers: one barrier per tile)
 #pragma unroll
             for (int l = 0; l < L; ++l) {
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) H[l][v] = __builtin_fmaf(A[l][v], h[v], H[l][v]);
             }
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) start[v] = h[v];
+        }
+        if (p.carry != nullptr && i0 % p.carry_len == 0 && i0 < p.T) {
+            float* c = p.carry + ((long long)w.b * p.carries + i0 / p.carry_len) * p.D + w.ch0;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                if (v < w.nch) c[v] = start[v];
         }
 #pragma unroll
         for (int l = 0; l < L; ++l) {
@@ -242,7 +353,7 @@ __global__ __launch_bounds__(S::NT) void scan_fwd_kernel(ScanArgs p) {
             float o[VEC];
 #pragma unroll
             for (int v = 0; v < VEC; ++v) o[v] = on ? H[l][v] : 0.f;
-            scan_store<T, VEC>(out + t * p.D, o, ow, w.nch);
+            scan_store<T, VEC, MODE>(out + t * p.D, o, w.nch);
         }
     }
     if (w.chunk == p.chunks - 1 && sub == 0) {
@@ -252,100 +363,92 @@ __global__ __launch_bounds__(S::NT) void scan_fwd_kernel(ScanArgs p) {
     }
 }
 
-template <typename T, typename S, bool LOGIT>
+template <typename T, typename S, bool LOGIT, bool MIX, int MODE>
 __global__ __launch_bounds__(S::NT) void scan_bwd_kernel(ScanArgs p) {
     constexpr int VEC = S::VEC, L = S::L, TILE = ScanTiles<S>::TILE;
     __shared__ float2 part[2][S::NT / 64 * S::CL * VEC];
     const ScanWhere w = scan_where<S>(p);
     const ScanTiles<S> tl(p, w.chunk);
-    const int sub = threadIdx.x / S::CL;
-    const bool xw = scan_wide<T, VEC>(p.x, p.xs, p.D) && w.nch > 0, gw = scan_wide<T, VEC>(p.gate, p.gs, p.D) && w.nch > 0,
-               dw = scan_wide<T, VEC>(p.dh, p.ds, p.D) && w.nch > 0, ow = p.D % VEC == 0;
+    const int sub = ScanLane<S>().sub;
     const T* x = (const T*)p.x + w.b * p.xs[0] + w.ch0 * p.xs[2];
     const T* g = (const T*)p.gate + w.b * p.gs[0] + w.ch0 * p.gs[2];
     const T* dh = (const T*)p.dh + w.b * p.ds[0] + w.ch0 * p.ds[2];
     const long long base = (long long)w.b * p.T * p.D + w.ch0;
+    Raw<T, VEC> xr[L], gr[L], dr[L];
+    float hin[VEC];
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+            const int i = tile * TILE + sub * L + l;
+            const bool on = i < w.n && w.nch > 0;
+            const long long t = p.reverse ? w.n - 1 - i : i;
+            if (on) {
+                gr[l] = scan_load<T, VEC, MODE != SCAN_ANY>(g + t * p.gs[1], p.gs[2], w.nch);
+                xr[l] = scan_load<T, VEC, MODE != SCAN_ANY>(x + t * p.xs[1], p.xs[2], w.nch);
+            } else {
+                gr[l] = scan_no_gate<T, VEC, LOGIT>();
+                xr[l] = scan_nothing<T, VEC>();
+            }
+            if (on && p.dh != nullptr) dr[l] = scan_load<T, VEC, MODE != SCAN_ANY>(dh + t * p.ds[1], p.ds[2], w.nch);
+            else dr[l] = scan_nothing<T, VEC>();
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v)
+            hin[v] = v < w.nch ? p.carry[((long long)w.b * p.carries + tile) * p.D + w.ch0 + v] : 0.f;
+    };
+    if (tl.last > tl.first) fetch(tl.last - 1);
     float rin[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) rin[v] = p.dlast && v < w.nch ? p.dlast[(long long)w.b * p.D + w.ch0 + v] : 0.f;
     scan_fold_chunks<S, false>(p, w, rin);
     for (int tile = tl.last - 1; tile >= tl.first; --tile) {
         const int i0 = tile * TILE + sub * L;
-        float dx[L][VEC], dg[L][VEC];
-        if (tile * TILE < w.n) {
-            Raw<T, VEC> xr[L], gr[L], dr[L];
-#pragma unroll
-            for (int l = 0; l < L; ++l) {
-                const int i = min(i0 + l, w.n - 1);
-                const long long t = p.reverse ? w.n - 1 - i : i;
-                gr[l] = scan_load<T, VEC>(g + t * p.gs[1], p.gs[2], gw, w.nch);
-                xr[l] = scan_load<T, VEC>(x + t * p.xs[1], p.xs[2], xw, w.nch);
-                if (p.dh != nullptr) {
-                    dr[l] = scan_load<T, VEC>(dh + t * p.ds[1], p.ds[2], dw, w.nch);
-                } else {
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) dr[l].e[v] = from_f32<T>(0.f);
-                }
-            }
-            float hin[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                hin[v] = v < w.nch ? p.carry[((long long)w.b * tl.tiles + tile) * p.D + w.ch0 + v] : 0.f;
-            // the tile's states again: prev[l] = the state in front of step l, first relative to the thread's start
-            float PA[L][VEC], prev[L][VEC], a[VEC], h[VEC];
+        // per step: G = q + P r_in, dx = G c or G, dgate = G wt
+        float P[L][VEC], q[L][VEC], wt[L][VEC], cc[L][VEC], a[VEC], h[VEC];
+        const bool some = tile * TILE < w.n;
+        if (some) {
             Gate ga[L][VEC];
+            // the tile's states again: wt = the state in front of step l (- x), first relative to the thread's start
 #pragma unroll
             for (int v = 0; v < VEC; ++v) { a[v] = 1.f; h[v] = 0.f; }
 #pragma unroll
             for (int l = 0; l < L; ++l) {
-                const bool on = i0 + l < w.n;
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    ga[l][v] = gate_of(to_f32(gr[l].e[v]), LOGIT);
-                    PA[l][v] = a[v];
-                    prev[l][v] = h[v];
-                    const float hv = scan_step(h[v], to_f32(xr[l].e[v]), ga[l][v], LOGIT, p.mix);
-                    const float av = decayed(a[v], ga[l][v], LOGIT);
-                    h[v] = on ? hv : h[v];
-                    a[v] = on ? av : a[v];
+                    const float xv = xr[l].get(v);
+                    ga[l][v] = gate_of<LOGIT>(gr[l].get(v));
+                    P[l][v] = a[v];
+                    wt[l][v] = MIX ? h[v] - xv : h[v];
+                    h[v] = scan_step<LOGIT, MIX>(h[v], xv, ga[l][v]);
+                    a[v] = decayed<LOGIT>(a[v], ga[l][v]);
                 }
             }
             scan_across<S, true>(a, h, hin, part[0]);
 #pragma unroll
             for (int l = 0; l < L; ++l) {
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) prev[l][v] = __builtin_fmaf(PA[l][v], h[v], prev[l][v]);
+                for (int v = 0; v < VEC; ++v) {
+                    wt[l][v] = __builtin_fmaf(P[l][v], h[v], wt[l][v]);
+                    if (LOGIT) wt[l][v] *= decayed<LOGIT>(ga[l][v].c, ga[l][v]);      // a c
+                }
             }
-            // r = a G, carried from later steps to earlier ones; PA and q relative to the thread's end
-            float q[L][VEC];
+            // r = a G, carried from later steps to earlier ones; P and q relative to the thread's end
 #pragma unroll
             for (int v = 0; v < VEC; ++v) { a[v] = 1.f; h[v] = 0.f; }
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
-                const bool on = i0 + l < w.n;
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    PA[l][v] = a[v];
-                    q[l][v] = h[v];
-                    const float hv = decayed(h[v] + to_f32(dr[l].e[v]), ga[l][v], LOGIT), av = decayed(a[v], ga[l][v], LOGIT);
-                    h[v] = on ? hv : h[v];
-                    a[v] = on ? av : a[v];
-                }
-            }
-            scan_across<S, false>(a, h, rin, part[1]);
-#pragma unroll
-            for (int l = 0; l < L; ++l) {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const float xv = to_f32(xr[l].e[v]);
-                    const float G = to_f32(dr[l].e[v]) + __builtin_fmaf(PA[l][v], h[v], q[l][v]);
-                    float da = G * (p.mix ? prev[l][v] - xv : prev[l][v]);
-                    if (LOGIT) da *= ga[l][v].a * ga[l][v].c;
-                    dx[l][v] = p.mix ? G * ga[l][v].c : G;
-                    dg[l][v] = da;
+                    P[l][v] = a[v];
+                    q[l][v] = h[v] + dr[l].get(v);
+                    h[v] = decayed<LOGIT>(q[l][v], ga[l][v]);
+                    a[v] = decayed<LOGIT>(a[v], ga[l][v]);
+                    if (MIX) cc[l][v] = ga[l][v].c;
                 }
             }
         }
+        if (tile > tl.first) fetch(tile - 1);       // in flight over the second scan and the stores
+        if (some) scan_across<S, false>(a, h, rin, part[1]);
 #pragma unroll
         for (int l = 0; l < L; ++l) {
             const int i = i0 + l;
@@ -354,9 +457,13 @@ __global__ __launch_bounds__(S::NT) void scan_bwd_kernel(ScanArgs p) {
             const long long t = on && p.reverse ? w.n - 1 - i : i;
             float ox[VEC], og[VEC];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) { ox[v] = on ? dx[l][v] : 0.f; og[v] = on ? dg[l][v] : 0.f; }
-            scan_store<T, VEC>((T*)p.dx + base + t * p.D, ox, ow, w.nch);
-            scan_store<T, VEC>((T*)p.dg + base + t * p.D, og, ow, w.nch);
+            for (int v = 0; v < VEC; ++v) {
+                const float G = __builtin_fmaf(P[l][v], h[v], q[l][v]);
+                ox[v] = on ? (MIX ? G * cc[l][v] : G) : 0.f;
+                og[v] = on ? G * wt[l][v] : 0.f;
+            }
+            scan_store<T, VEC, MODE>((T*)p.dx + base + t * p.D, ox, w.nch);
+            scan_store<T, VEC, MODE>((T*)p.dg + base + t * p.D, og, w.nch);
         }
     }
     if (w.chunk == 0 && sub == 0) {
@@ -368,21 +475,18 @@ __global__ __launch_bounds__(S::NT) void scan_bwd_kernel(ScanArgs p) {
 
 // Product of gates and end state of every chunk, from 0 (forward: UP) or of the gradient's recurrence (r = a (dh + r)).
 // A thread walks a run of its own through the chunk; the runs are joined once.
-template <typename T, typename S, bool LOGIT, bool UP>
+template <typename T, typename S, bool LOGIT, bool MIX, bool UP, int MODE>
 __global__ __launch_bounds__(S::NT) void scan_sum_kernel(ScanArgs p) {
-    constexpr int VEC = S::VEC, TILE = ScanTiles<S>::TILE, SUB = ScanTiles<S>::SUB, U = 4;
+    constexpr int VEC = S::VEC, SUB = ScanTiles<S>::SUB, U = 4;
     __shared__ float2 part[S::NT / 64 * S::CL * VEC];
     const ScanWhere w = scan_where<S>(p);
-    const ScanTiles<S> tl(p, w.chunk);
-    const int sub = threadIdx.x / S::CL;
+    const int sub = ScanLane<S>().sub;
     const T* v1 = UP ? (const T*)p.x : (const T*)p.dh;
     const long long s0 = UP ? p.xs[0] : p.ds[0], s1 = UP ? p.xs[1] : p.ds[1], s2 = UP ? p.xs[2] : p.ds[2];
-    const bool vw = (UP ? scan_wide<T, VEC>(p.x, p.xs, p.D) : scan_wide<T, VEC>(p.dh, p.ds, p.D)) && w.nch > 0;
-    const bool gw = scan_wide<T, VEC>(p.gate, p.gs, p.D) && w.nch > 0;
     const T* g = (const T*)p.gate + w.b * p.gs[0] + w.ch0 * p.gs[2];
     v1 += w.b * s0 + w.ch0 * s2;
-    const int begin = tl.first * TILE, end = min(tl.last * TILE, w.n), run = (max(end - begin, 0) + SUB - 1) / SUB;
-    const int i0 = begin + sub * run, i1 = min(i0 + run, end);
+    const int begin = min(w.chunk * p.chunk_len, p.T), end = min(min(begin + p.chunk_len, p.T), w.n), run = (max(end - begin, 0) + SUB - 1) / SUB;
+    const int i0 = begin + sub * run, i1 = w.nch > 0 ? min(i0 + run, end) : i0;
     float a[VEC], h[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { a[v] = 1.f; h[v] = 0.f; }
@@ -392,12 +496,12 @@ __global__ __launch_bounds__(S::NT) void scan_sum_kernel(ScanArgs p) {
         for (int u = 0; u < U; ++u) {
             const int j = min(k + u, i1 - 1), i = UP ? j : i0 + (i1 - 1 - j);
             const long long t = p.reverse ? w.n - 1 - i : i;
-            gr[u] = scan_load<T, VEC>(g + t * p.gs[1], p.gs[2], gw, w.nch);
+            gr[u] = scan_load<T, VEC, MODE != SCAN_ANY>(g + t * p.gs[1], p.gs[2], w.nch);
             if (UP || p.dh != nullptr) {
-                vr[u] = scan_load<T, VEC>(v1 + t * s1, s2, vw, w.nch);
+                vr[u] = scan_load<T, VEC, MODE != SCAN_ANY>(v1 + t * s1, s2, w.nch);
             } else {
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) vr[u].e[v] = from_f32<T>(0.f);
+                for (int v = 0; v < VEC; ++v) vr[u].put(v, from_f32<T>(0.f));
             }
         }
 #pragma unroll
@@ -405,31 +509,25 @@ __global__ __launch_bounds__(S::NT) void scan_sum_kernel(ScanArgs p) {
             const bool on = k + u < i1;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const Gate ga = gate_of(to_f32(gr[u].e[v]), LOGIT);
-                const float xv = to_f32(vr[u].e[v]);
-                const float hv = UP ? scan_step(h[v], xv, ga, LOGIT, p.mix) : decayed(h[v] + xv, ga, LOGIT);
-                const float av = decayed(a[v], ga, LOGIT);
+                const Gate ga = gate_of<LOGIT>(gr[u].get(v));
+                const float xv = vr[u].get(v);
+                const float hv = UP ? scan_step<LOGIT, MIX>(h[v], xv, ga) : decayed<LOGIT>(h[v] + xv, ga);
+                const float av = decayed<LOGIT>(a[v], ga);
                 h[v] = on ? hv : h[v];
                 a[v] = on ? av : a[v];
             }
         }
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cl = threadIdx.x % S::CL;
+    constexpr int SW = ScanLane<S>::SW;
+    const int wave = threadIdx.x >> 6, cl = ScanLane<S>().cl, li = threadIdx.x & (SW - 1);
 #pragma unroll
-    for (int o = S::CL; o < 64; o <<= 1) {      // thread s takes in the o / CL threads in front of it (UP) or behind it
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const float pa = UP ? __shfl_up(a[v], o, 64) : __shfl_down(a[v], o, 64);
-            const float ph = UP ? __shfl_up(h[v], o, 64) : __shfl_down(h[v], o, 64);
-            if (UP ? lane >= o : lane < 64 - o) SCAN_JOIN(a[v], h[v], pa, ph);
-        }
-    }
-    if (UP ? lane >= 64 - S::CL : lane < S::CL) {
+    for (int v = 0; v < VEC; ++v) scan_lanes<SW, UP>(a[v], h[v]);
+    if (li == (UP ? SW - 1 : 0)) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) part[wave * S::CL * VEC + cl * VEC + v] = make_float2(a[v], h[v]);
     }
     __syncthreads();
-    if ((int)threadIdx.x < S::CL) {
+    if (wave == 0 && li == 0) {
         float* out = p.sums + ((long long)w.b * p.chunks + w.chunk) * 2 * p.D + w.ch0;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -446,21 +544,30 @@ __global__ __launch_bounds__(S::NT) void scan_sum_kernel(ScanArgs p) {
 }
 
 // How a problem is cut (the forward and the backward pass of one call agree on it: a function of the sizes alone).
-struct ScanPlan { int row, tile, tiles, slabs, chunks; };
+struct ScanPlan { int row, slabs, chunks, chunk_len, carry_len, carries; };
+template <typename F, typename B>
+static void scan_cut(ScanPlan& k, long long groups, int T) {
+    const int tile = ScanTiles<F>::TILE, tiles = (T + tile - 1) / tile;
+    static_assert(ScanTiles<F>::TILE % ScanTiles<B>::TILE == 0, "whole backward tiles");
+    k.carry_len = ScanTiles<B>::TILE;
+    k.carries = (T + k.carry_len - 1) / k.carry_len;
+    long long want = groups > 0 && groups < SC_TARGET ? (512 + groups - 1) / groups : 1;
+    if (want > tiles) want = tiles;
+    if (want > 64) want = 64;
+    if (want < 1) want = 1;
+    const int per = (int)((tiles + want - 1) / want);
+    k.chunks = per > 0 ? (tiles + per - 1) / per : 1;
+    k.chunk_len = per > 0 ? per * tile : tile;
+}
 static ScanPlan scan_plan(int B, int T, int D, int dtype) {
     ScanPlan k;
     k.row = D < 8;
-    const int width = k.row ? 1 : (dtype == SEQ_F32 ? 16 : 32);
-    k.tile = k.row ? ScanRow::NT * ScanRow::L : (dtype == SEQ_F32 ? 64 * ScanShape<elem_f32>::L : 64 * ScanShape<elem_bf16>::L);
-    k.tiles = (T + k.tile - 1) / k.tile;
+    const int width = k.row ? 1 : SCAN_CL * (dtype == SEQ_F32 ? 4 : 8);
     k.slabs = (D + width - 1) / width;
     const long long groups = (long long)B * k.slabs;
-    k.chunks = 1;
-    if (groups < 256 && k.tiles > 1) {
-        const long long want = (512 + groups - 1) / groups;
-        k.chunks = (int)(want < k.tiles ? want : k.tiles);
-        if (k.chunks > 64) k.chunks = 64;
-    }
+    if (k.row) scan_cut<ScanRow, ScanRow>(k, groups, T);
+    else if (dtype == SEQ_F32) scan_cut<ScanFwd<elem_f32>, ScanBwd<elem_f32>>(k, groups, T);
+    else scan_cut<ScanFwd<elem_bf16>, ScanBwd<elem_bf16>>(k, groups, T);
     return k;
 }
 
@@ -468,42 +575,58 @@ static bool scan_ok(const ScanArgs& p) {
     return p.B >= 0 && p.T >= 0 && p.D >= 0 && (long long)p.B * p.D < (1ll << 31) && (unsigned)p.T < (1u << 30);
 }
 
-// tiles and chunks of a problem: the caller's carry is [B][tiles][D], its sums [B][chunks][2][D] floats
-PDA_EXPORT int pda_scan_plan(int B, int T, int D, int dtype, int* tiles, int* chunks) {
+// what the caller allocates: carry is [B][carries][D] floats, sums [B][chunks][2][D] (chunks > 1)
+PDA_EXPORT int pda_scan_plan(int B, int T, int D, int dtype, int* carries, int* chunks) {
+    if (B < 0 || T < 0 || D < 0 || (unsigned)T >= (1u << 30) || dtype < SEQ_F32 || dtype > SEQ_F16) return SEQ_REFUSED;
     const ScanPlan k = scan_plan(B, T, D, dtype);
-    *tiles = k.tiles;
+    *carries = k.carries;
     *chunks = k.chunks;
     return 0;
 }
 
-template <typename T, typename S, bool LOGIT>
+template <typename T, typename F, typename B, bool LOGIT, bool MIX, int MODE>
 static void scan_launch(const ScanArgs& p, const ScanPlan& k, bool backward, hipStream_t stream) {
-    const dim3 grid((unsigned)((long long)p.B * k.slabs * k.chunks)), block(S::NT);
+    constexpr int READ = MODE == SCAN_STREAM ? SCAN_WIDE : MODE;
+    const dim3 grid((unsigned)((long long)p.B * k.slabs * k.chunks)), fwd(F::NT), bwd(B::NT);
     if (!backward) {
-        if (k.chunks > 1) hipLaunchKernelGGL((scan_sum_kernel<T, S, LOGIT, true>), grid, block, 0, stream, p);
-        hipLaunchKernelGGL((scan_fwd_kernel<T, S, LOGIT>), grid, block, 0, stream, p);
+        if (k.chunks > 1) hipLaunchKernelGGL((scan_sum_kernel<T, F, LOGIT, MIX, true, READ>), grid, fwd, 0, stream, p);
+        hipLaunchKernelGGL((scan_fwd_kernel<T, F, LOGIT, MIX, MODE>), grid, fwd, 0, stream, p);
     } else {
-        if (k.chunks > 1) hipLaunchKernelGGL((scan_sum_kernel<T, S, LOGIT, false>), grid, block, 0, stream, p);
-        hipLaunchKernelGGL((scan_bwd_kernel<T, S, LOGIT>), grid, block, 0, stream, p);
+        if (k.chunks > 1) hipLaunchKernelGGL((scan_sum_kernel<T, B, LOGIT, false, false, READ>), grid, bwd, 0, stream, p);
+        hipLaunchKernelGGL((scan_bwd_kernel<T, B, LOGIT, MIX, MODE>), grid, bwd, 0, stream, p);
     }
+}
+template <typename T, typename F, typename B, int MODE>
+static void scan_forms(const ScanArgs& p, const ScanPlan& k, bool backward, hipStream_t stream) {
+    if (p.logit && p.mix) scan_launch<T, F, B, true, true, MODE>(p, k, backward, stream);
+    else if (p.logit) scan_launch<T, F, B, true, false, MODE>(p, k, backward, stream);
+    else if (p.mix) scan_launch<T, F, B, false, true, MODE>(p, k, backward, stream);
+    else scan_launch<T, F, B, false, false, MODE>(p, k, backward, stream);
+}
+static bool scan_wide(const void* base, const long long* s, int D, int vec) {
+    return s[2] == 1 && D % vec == 0 && s[0] % vec == 0 && s[1] % vec == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0;
 }
 template <typename T>
 static void scan_dispatch(const ScanArgs& p, const ScanPlan& k, bool backward, hipStream_t stream) {
-    if (k.row) {
-        if (p.logit) scan_launch<T, ScanRow, true>(p, k, backward, stream);
-        else scan_launch<T, ScanRow, false>(p, k, backward, stream);
-    } else {
-        if (p.logit) scan_launch<T, ScanShape<T>, true>(p, k, backward, stream);
-        else scan_launch<T, ScanShape<T>, false>(p, k, backward, stream);
-    }
+    constexpr int VEC = 16 / sizeof(T);
+    const bool wide = scan_wide(p.x, p.xs, p.D, VEC) && scan_wide(p.gate, p.gs, p.D, VEC) &&
+                      (!backward || p.dh == nullptr || scan_wide(p.dh, p.ds, p.D, VEC));
+    if (k.row) scan_forms<T, ScanRow, ScanRow, SCAN_ANY>(p, k, backward, stream);
+    else if (!wide) scan_forms<T, ScanFwd<T>, ScanBwd<T>, SCAN_ANY>(p, k, backward, stream);
+    else if (seq_streams((long long)p.B * p.T * p.D * (long long)sizeof(T)))
+        scan_forms<T, ScanFwd<T>, ScanBwd<T>, SCAN_STREAM>(p, k, backward, stream);
+    else scan_forms<T, ScanFwd<T>, ScanBwd<T>, SCAN_WIDE>(p, k, backward, stream);
 }
 static int scan_run(const ScanArgs* args, int dtype, bool backward, hipStream_t stream) {
     ScanArgs p = *args;
     if (!scan_ok(p) || dtype < SEQ_F32 || dtype > SEQ_F16) return SEQ_REFUSED;
     if ((long long)p.B * p.D == 0) return 0;
     const ScanPlan k = scan_plan(p.B, p.T, p.D, dtype);
-    if (p.chunks != k.chunks || (k.chunks > 1 && p.sums == nullptr) || (backward && k.tiles > 0 && p.carry == nullptr))
+    if (p.chunks != k.chunks || (k.chunks > 1 && p.sums == nullptr) || (backward && k.carries > 0 && p.carry == nullptr))
         return SEQ_REFUSED;
+    p.chunk_len = k.chunk_len;
+    p.carry_len = k.carry_len;
+    p.carries = k.carries;
     if ((long long)p.B * k.slabs * k.chunks >= (1ll << 31) / ScanRow::NT * 2) return SEQ_REFUSED;
     if (dtype == SEQ_F32) scan_dispatch<elem_f32>(p, k, backward, stream);
     else if (dtype == SEQ_BF16) scan_dispatch<elem_bf16>(p, k, backward, stream);
@@ -518,26 +641,33 @@ struct ScanStepArgs {
     long long xs[2], gs[2], ss[2], os[2];       // element strides (request, channel)
     int B, D, logit, mix;
 };
-template <typename T>
+template <typename T, bool LOGIT, bool MIX>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanStepArgs p) {
     const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
     if (id >= (long long)p.B * p.D) return;
     const int b = (int)(id / p.D), d = (int)(id - (long long)b * p.D);
     const float x = to_f32(((const T*)p.x)[b * p.xs[0] + d * p.xs[1]]);
-    const Gate g = gate_of(to_f32(((const T*)p.gate)[b * p.gs[0] + d * p.gs[1]]), p.logit);
-    const float h = scan_step(p.state[b * p.ss[0] + d * p.ss[1]], x, g, p.logit, p.mix);
+    const Gate g = gate_of<LOGIT>(to_f32(((const T*)p.gate)[b * p.gs[0] + d * p.gs[1]]));
+    float h = scan_step<LOGIT, MIX>(p.state[b * p.ss[0] + d * p.ss[1]], x, g);
+    asm("" : "+v"(h));          // what is returned is the stored state rounded, not a second rounding of the exact one
     p.state_out[b * p.os[0] + d * p.os[1]] = h;
     ((T*)p.h)[id] = from_f32<T>(h);
 }
-
+template <typename T>
+static void scan_step_launch(const ScanStepArgs& p, hipStream_t stream) {
+    const dim3 grid((unsigned)(((long long)p.B * p.D + 255) / 256)), block(256);
+    if (p.logit && p.mix) hipLaunchKernelGGL((scan_step_kernel<T, true, true>), grid, block, 0, stream, p);
+    else if (p.logit) hipLaunchKernelGGL((scan_step_kernel<T, true, false>), grid, block, 0, stream, p);
+    else if (p.mix) hipLaunchKernelGGL((scan_step_kernel<T, false, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((scan_step_kernel<T, false, false>), grid, block, 0, stream, p);
+}
 PDA_EXPORT int pda_scan_step(const ScanStepArgs* args, int dtype, hipStream_t stream) {
     const ScanStepArgs p = *args;
     if (p.B < 0 || p.D < 0 || (long long)p.B * p.D >= (1ll << 31)) return SEQ_REFUSED;
     if ((long long)p.B * p.D == 0) return 0;
-    const dim3 grid((unsigned)(((long long)p.B * p.D + 255) / 256)), block(256);
-    if (dtype == SEQ_F32) hipLaunchKernelGGL(scan_step_kernel<elem_f32>, grid, block, 0, stream, p);
-    else if (dtype == SEQ_BF16) hipLaunchKernelGGL(scan_step_kernel<elem_bf16>, grid, block, 0, stream, p);
-    else if (dtype == SEQ_F16) hipLaunchKernelGGL(scan_step_kernel<elem_f16>, grid, block, 0, stream, p);
+    if (dtype == SEQ_F32) scan_step_launch<elem_f32>(p, stream);
+    else if (dtype == SEQ_BF16) scan_step_launch<elem_bf16>(p, stream);
+    else if (dtype == SEQ_F16) scan_step_launch<elem_f16>(p, stream);
     else return SEQ_REFUSED;
     return seq_launched();
 }

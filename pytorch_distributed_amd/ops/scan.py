@@ -19,7 +19,8 @@ class _Args(ctypes.Structure):      # mirrors ScanArgs in csrc/scan.hip
     _fields_ = [("x", _vp), ("gate", _vp), ("dh", _vp), ("xs", _i64 * 3), ("gs", _i64 * 3), ("ds", _i64 * 3), ("h0", _vp),
                 ("dlast", _vp), ("lengths", _vp), ("len64", _int), ("h", _vp), ("last", _vp), ("carry", _vp),
                 ("sums", _vp), ("dx", _vp), ("dg", _vp), ("dh0", _vp), ("B", _int), ("T", _int), ("D", _int),
-                ("logit", _int), ("mix", _int), ("reverse", _int), ("chunks", _int)]
+                ("logit", _int), ("mix", _int), ("reverse", _int), ("chunks", _int), ("chunk_len", _int),
+                ("carry_len", _int), ("carries", _int)]
 
 
 class _StepArgs(ctypes.Structure):  # mirrors ScanStepArgs
@@ -84,7 +85,7 @@ def _backward_torch(x, gate, h0, n, logit, mix, reverse, dh, dlast):
 
 
 def _plan(x):
-    """-> (tiles, chunks): how the kernels cut x's steps (csrc/scan.hip scan_plan)"""
+    """-> (carries, chunks): how the kernels cut x's steps (csrc/scan.hip scan_plan)"""
     out = (ctypes.c_int * 2)()
     B, T, D = x.shape
     native("pda_scan_plan")(B, T, D, TYPE_CODES[x.dtype], ctypes.byref(out, 0), ctypes.byref(out, 4))
@@ -117,9 +118,9 @@ class _LinearScan(torch.autograd.Function):
             h = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
             last = torch.empty(B, D, dtype=torch.float32, device=x.device)
             args = _fill(_Args(), x, gate, h0, lengths, how)
-            tiles, args.chunks = _plan(x)
+            carries, args.chunks = _plan(x)
             if any(ctx.needs_input_grad):
-                carry = torch.empty(B, tiles, D, dtype=torch.float32, device=x.device)
+                carry = torch.empty(B, carries, D, dtype=torch.float32, device=x.device)
             if args.chunks > 1:
                 sums = torch.empty(B, args.chunks, 2, D, dtype=torch.float32, device=x.device)
                 args.sums = ptr(sums)
