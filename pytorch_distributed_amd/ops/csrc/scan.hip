@@ -59,22 +59,13 @@ __device__ __forceinline__ int scan_length(const ScanArgs& p, int b) {
 // Where the slabs do not fill the card, the steps are cut into chunks: scan_sum_kernel leaves every chunk's product of
 // gates and end state, and each chunk's workgroup folds those in front of it before it starts.  x and gate are then read
 // twice.
-#ifndef SC_FL
-#define SC_FNT 512
-#define SC_FL 4
-#define SC_BNT 256
-#define SC_BL 4
-#endif
-#ifndef SCAN_CL
 #define SCAN_CL 8
-#endif
-#ifndef SC_TARGET
-#define SC_TARGET 256
-#endif
 // a forward tile holds a whole number of backward tiles: the forward pass leaves the state in front of each of those
-template <typename T> struct ScanFwd { static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = SC_FL * 8 / VEC, NT = SC_FNT; };
-template <typename T> struct ScanBwd { static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = SC_BL * 8 / VEC, NT = SC_BNT; };
-struct ScanRow { static constexpr int VEC = 1, CL = 1, L = 8, NT = 1024; };     // few channels: one per workgroup
+template <typename T> struct ScanFwd { static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = 32 / VEC, NT = 512; };
+template <typename T> struct ScanBwd { static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = 32 / VEC, NT = 256; };
+// fewer than 8 channels: one sequence of one channel per workgroup, of 16 waves or of one
+struct ScanRow { static constexpr int VEC = 1, CL = 1, L = 8, NT = 1024; };
+struct ScanWave { static constexpr int VEC = 1, CL = 1, L = 8, NT = 64; };
 // The lanes of a wave: SW consecutive ones hold consecutive runs of steps of one group of VEC channels, so that a scan
 // over steps moves along a DPP row.
 template <typename S> struct ScanLane {
@@ -94,11 +85,7 @@ template <typename S>
 __device__ __forceinline__ ScanWhere scan_where(const ScanArgs& p) {
     const int nslab = (p.D + S::CL * S::VEC - 1) / (S::CL * S::VEC);
     ScanWhere w;
-#ifdef SC_XCD
-    const int n8 = (int)gridDim.x / 8, id = (int)blockIdx.x < n8 * 8 ? ((int)blockIdx.x & 7) * n8 + ((int)blockIdx.x >> 3) : (int)blockIdx.x;
-#else
     const int id = blockIdx.x;
-#endif
     const int rest = id / nslab;
     w.ch0 = ((id - rest * nslab) * S::CL + ScanLane<S>().cl) * S::VEC;
     w.nch = min(max(p.D - w.ch0, 0), S::VEC);
@@ -158,42 +145,49 @@ __device__ __forceinline__ float dpp_shift(float none, float v) {       // lane 
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
                                                                  (UP ? 0x110 : 0x100) + O, 0xf, BANKS, false));
 }
+template <bool UP>
+__device__ __forceinline__ float wave_shift(float v) {                  // lane i of the wave gets lane i -+ 1's
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), UP ? 0x138 : 0x130, 0xf, 0xf, false));
+}
 template <int O, int SW, bool UP>
 __device__ __forceinline__ void scan_lanes_step(float& A, float& H) {
     if constexpr (O < SW) {
-        const int i = threadIdx.x & (SW - 1);
-        const bool on = UP ? i >= O : i < SW - O;
-        float pa, ph;
-        if constexpr (O < 16) {
-            constexpr int BANKS = SW == 8 && O == 4 ? (UP ? 0xa : 0x5) : 0xf;      // (the lanes of a group that have a partner)
-            pa = dpp_shift<O, UP, BANKS>(1.f, A);
-            ph = dpp_shift<O, UP, BANKS>(0.f, H);
-            if (SW < 16 && BANKS == 0xf) { pa = on ? pa : 1.f; ph = on ? ph : 0.f; }
-        } else {
-            pa = UP ? __shfl_up(A, O, 64) : __shfl_down(A, O, 64);
-            ph = UP ? __shfl_up(H, O, 64) : __shfl_down(H, O, 64);
+        constexpr int BANKS = SW == 8 && O == 4 ? (UP ? 0xa : 0x5) : 0xf;      // (the lanes of a group that have a partner)
+        float pa = dpp_shift<O, UP, BANKS>(1.f, A), ph = dpp_shift<O, UP, BANKS>(0.f, H);
+        if (SW < 16 && BANKS == 0xf) {
+            const int i = threadIdx.x & (SW - 1);
+            const bool on = UP ? i >= O : i < SW - O;
             pa = on ? pa : 1.f;
             ph = on ? ph : 0.f;
-        }
-        if constexpr (SW > 16 && O < 16) {      // rows of 16 are joined by the steps of 16 and 32: a wave's lanes in order
-            const int r = threadIdx.x & 15;
-            const float qa = UP ? __shfl_up(A, O, 64) : __shfl_down(A, O, 64), qh = UP ? __shfl_up(H, O, 64) : __shfl_down(H, O, 64);
-            const bool over = UP ? r < O : r >= 16 - O;
-            pa = over && on ? qa : pa;
-            ph = over && on ? qh : ph;
         }
         SCAN_JOIN(A, H, pa, ph);
     }
 }
+__device__ __forceinline__ float scan_lane(float v, int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
 // inclusive over the SW lanes of a channel group
 template <int SW, bool UP>
 __device__ __forceinline__ void scan_lanes(float& A, float& H) {
+    static_assert(SW == 8 || SW == 16 || SW == 64, "");
     scan_lanes_step<1, SW, UP>(A, H);
     scan_lanes_step<2, SW, UP>(A, H);
     scan_lanes_step<4, SW, UP>(A, H);
     scan_lanes_step<8, SW, UP>(A, H);
-    scan_lanes_step<16, SW, UP>(A, H);
-    scan_lanes_step<32, SW, UP>(A, H);
+    if constexpr (SW == 64) {       // the four rows of 16
+        const int row = (threadIdx.x >> 4) & 3, at = UP ? row : 3 - row;
+        float pa = 1.f, ph = 0.f, ta = 1.f, th = 0.f;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const int end = UP ? 16 * k + 15 : 48 - 16 * k;
+            const float a = scan_lane(A, end), h = scan_lane(H, end);
+            th = __builtin_fmaf(a, th, h);
+            ta *= a;
+            pa = at > k ? ta : pa;
+            ph = at > k ? th : ph;
+        }
+        SCAN_JOIN(A, H, pa, ph);
+    }
 }
 template <typename S, bool UP>
 __device__ __forceinline__ void scan_across(float (&A)[S::VEC], float (&H)[S::VEC], float (&in)[S::VEC], float2* part) {
@@ -213,8 +207,8 @@ __device__ __forceinline__ void scan_across(float (&A)[S::VEC], float (&H)[S::VE
             pa = dpp_shift<1, UP>(1.f, A[v]);
             ph = dpp_shift<1, UP>(0.f, H[v]);
         } else {
-            pa = UP ? __shfl_up(A[v], 1, 64) : __shfl_down(A[v], 1, 64);
-            ph = UP ? __shfl_up(H[v], 1, 64) : __shfl_down(H[v], 1, 64);
+            pa = wave_shift<UP>(A[v]);
+            ph = wave_shift<UP>(H[v]);
         }
         A[v] = first ? 1.f : pa;
         H[v] = first ? 0.f : ph;
@@ -543,16 +537,24 @@ __global__ __launch_bounds__(S::NT) void scan_sum_kernel(ScanArgs p) {
     }
 }
 
+#ifndef SCAN_CHUNK_TILES
+#define SCAN_CHUNK_TILES 4
+#endif
 // How a problem is cut (the forward and the backward pass of one call agree on it: a function of the sizes alone).
-struct ScanPlan { int row, slabs, chunks, chunk_len, carry_len, carries; };
+struct ScanPlan { int kind, slabs, chunks, chunk_len, carry_len, carries; };
+#define SCAN_KIND_SLAB 0
+#define SCAN_KIND_ROW 1
+#define SCAN_KIND_WAVE 2
 template <typename F, typename B>
 static void scan_cut(ScanPlan& k, long long groups, int T) {
-    const int tile = ScanTiles<F>::TILE, tiles = (T + tile - 1) / tile;
     static_assert(ScanTiles<F>::TILE % ScanTiles<B>::TILE == 0, "whole backward tiles");
+    const int tile = ScanTiles<F>::TILE, tiles = (T + tile - 1) / tile;
     k.carry_len = ScanTiles<B>::TILE;
     k.carries = (T + k.carry_len - 1) / k.carry_len;
-    long long want = groups > 0 && groups < SC_TARGET ? (512 + groups - 1) / groups : 1;
-    if (want > tiles) want = tiles;
+    // chunks of at least SCAN_CHUNK_TILES tiles where the workgroups would leave CUs idle: below that the second reading
+    // and its launch take longer than the tiles that they save
+    long long want = groups > 0 && groups < 256 ? (512 + groups - 1) / groups : 1;
+    if (want > tiles / SCAN_CHUNK_TILES) want = tiles / SCAN_CHUNK_TILES;
     if (want > 64) want = 64;
     if (want < 1) want = 1;
     const int per = (int)((tiles + want - 1) / want);
@@ -561,11 +563,12 @@ static void scan_cut(ScanPlan& k, long long groups, int T) {
 }
 static ScanPlan scan_plan(int B, int T, int D, int dtype) {
     ScanPlan k;
-    k.row = D < 8;
-    const int width = k.row ? 1 : SCAN_CL * (dtype == SEQ_F32 ? 4 : 8);
+    const int width = D < 8 ? 1 : SCAN_CL * (dtype == SEQ_F32 ? 4 : 8);
     k.slabs = (D + width - 1) / width;
     const long long groups = (long long)B * k.slabs;
-    if (k.row) scan_cut<ScanRow, ScanRow>(k, groups, T);
+    k.kind = D >= 8 ? SCAN_KIND_SLAB : (T <= 4 * ScanTiles<ScanWave>::TILE || groups >= 1024) ? SCAN_KIND_WAVE : SCAN_KIND_ROW;
+    if (k.kind == SCAN_KIND_ROW) scan_cut<ScanRow, ScanRow>(k, groups, T);
+    else if (k.kind == SCAN_KIND_WAVE) scan_cut<ScanWave, ScanWave>(k, groups, T);
     else if (dtype == SEQ_F32) scan_cut<ScanFwd<elem_f32>, ScanBwd<elem_f32>>(k, groups, T);
     else scan_cut<ScanFwd<elem_bf16>, ScanBwd<elem_bf16>>(k, groups, T);
     return k;
@@ -611,7 +614,8 @@ static void scan_dispatch(const ScanArgs& p, const ScanPlan& k, bool backward, h
     constexpr int VEC = 16 / sizeof(T);
     const bool wide = scan_wide(p.x, p.xs, p.D, VEC) && scan_wide(p.gate, p.gs, p.D, VEC) &&
                       (!backward || p.dh == nullptr || scan_wide(p.dh, p.ds, p.D, VEC));
-    if (k.row) scan_forms<T, ScanRow, ScanRow, SCAN_ANY>(p, k, backward, stream);
+    if (k.kind == SCAN_KIND_ROW) scan_forms<T, ScanRow, ScanRow, SCAN_ANY>(p, k, backward, stream);
+    else if (k.kind == SCAN_KIND_WAVE) scan_forms<T, ScanWave, ScanWave, SCAN_ANY>(p, k, backward, stream);
     else if (!wide) scan_forms<T, ScanFwd<T>, ScanBwd<T>, SCAN_ANY>(p, k, backward, stream);
     else if (seq_streams((long long)p.B * p.T * p.D * (long long)sizeof(T)))
         scan_forms<T, ScanFwd<T>, ScanBwd<T>, SCAN_STREAM>(p, k, backward, stream);
@@ -627,7 +631,7 @@ static int scan_run(const ScanArgs* args, int dtype, bool backward, hipStream_t 
     p.chunk_len = k.chunk_len;
     p.carry_len = k.carry_len;
     p.carries = k.carries;
-    if ((long long)p.B * k.slabs * k.chunks >= (1ll << 31) / ScanRow::NT * 2) return SEQ_REFUSED;
+    if ((long long)p.B * k.slabs * k.chunks >= (1ll << 32) / ScanFwd<elem_f32>::NT) return SEQ_REFUSED;    // (a launch's threads)
     if (dtype == SEQ_F32) scan_dispatch<elem_f32>(p, k, backward, stream);
     else if (dtype == SEQ_BF16) scan_dispatch<elem_bf16>(p, k, backward, stream);
     else scan_dispatch<elem_f16>(p, k, backward, stream);

@@ -11,7 +11,7 @@ import ctypes
 import torch
 import torch.nn as nn
 
-from ._seq import TYPE_CODES, check_floating, launched, native, on_device, ptr, stream_of
+from ._seq import check_floating, native, ptr, run_on
 
 _M64 = (1 << 64) - 1
 _GOLDEN = 0x9E3779B97F4A7C15
@@ -65,17 +65,16 @@ def _run(x, residual, p, seed, site, counter, used):
         return (y if residual is None else y + residual.float()).to(x.dtype)
     entry = native("pda_dropout")
     hi, lo = _threshold(p)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)
     args = _Args(ptr(x), ptr(residual), ptr(y), ptr(counter), ptr(used), seed & _M64, site, hi, lo, scale, x.numel())
-    with on_device(x):
-        launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "dropout")
+    run_on(x, entry, "dropout", args)
     return y
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, site, counter):
-        used = torch.empty_like(counter)
+        used = torch.empty_like(counter) if any(ctx.needs_input_grad) else None
         y = _run(x.contiguous(), residual.contiguous() if residual is not None else None, p, seed, site, counter, used)
         ctx.save_for_backward(used)
         ctx.how = (p, seed, site)

@@ -11,7 +11,7 @@ from collections import namedtuple
 
 import torch
 
-from ._seq import TYPE_CODES, check_floating, check_int, launched, native, on_device, ptr, stream_of
+from ._seq import check_floating, check_int, native, ptr, run_on
 
 MAX_TOP = 32        # csrc/logprob.hip LP_MAX_TOP
 TokenLogprobs = namedtuple("TokenLogprobs", "logprob, entropy, logsumexp, top_logprobs, top_tokens")
@@ -68,57 +68,56 @@ def _backward_torch(x, tokens, m, ls, ent, d_lp, d_ent, d_lse, inv_t, ignore):
     return torch.where(off[:, None], torch.zeros_like(g), g).to(x.dtype)
 
 
-def _fill(args, x, tokens, inv_t, ignore):
-    args.logits, args.ld, args.rows, args.vocab = ptr(x), x.stride(0), x.shape[0], x.shape[1]
-    args.tokens, args.tok64, args.ignore, args.inv_t = ptr(tokens), int(tokens.dtype == torch.int64), ignore, inv_t
-    args.c = inv_t * _LOG2E
-    return args
-
-
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tokens, inv_t, top_k, ignore):
         n = x.shape[0]
         if x.device.type == "cpu":
             lp, ent, lse, m, ls, top, ids = _forward_torch(x, tokens, inv_t, top_k, ignore)
+            stat = torch.stack([m, ls])
         else:
             entry = native("pda_logprob")
-            lp, ent, lse, m, ls = (torch.empty(n, dtype=torch.float32, device=x.device) for _ in range(5))
-            top = torch.empty(n, top_k, dtype=torch.float32, device=x.device)
-            ids = torch.empty(n, top_k, dtype=torch.int64, device=x.device)
-            args = _fill(_Args(), x, tokens, inv_t, ignore)
-            args.logprob, args.entropy, args.lse, args.stat_m, args.stat_l2 = map(ptr, (lp, ent, lse, m, ls))
-            args.top_lp, args.top_id, args.top_k = ptr(top), ptr(ids), top_k
-            args.splits = native("pda_logprob_splits")(_i64(n), x.shape[1], top_k)
-            if args.splits > 1:     # long rows in parts, joined by a second launch
-                stat = torch.empty(n, args.splits, 4, dtype=torch.float32, device=x.device)
-                keys = torch.empty(n, args.splits, top_k, dtype=torch.int64, device=x.device)
-                args.part_stat, args.part_top = ptr(stat), ptr(keys)
-            with on_device(x):
-                launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "token_logprobs")
-        ctx.save_for_backward(x, tokens, m, ls, ent)
+            kw = {"dtype": torch.float32, "device": x.device}
+            lp, ent, lse, stat = torch.empty(n, **kw), torch.empty(n, **kw), torch.empty(n, **kw), torch.empty(2, n, **kw)
+            top = torch.empty(n, top_k, **kw) if top_k else None
+            ids = torch.empty(n, top_k, dtype=torch.int64, device=x.device) if top_k else None
+            v = x.shape[1]
+            splits = native("pda_logprob_splits")(_i64(n), v, top_k) if v > 1024 else 1
+            part = keys = None
+            if splits > 1:      # long rows in parts, joined by a second launch
+                part = torch.empty(n, splits, 4, **kw)
+                keys = torch.empty(n, splits, top_k, dtype=torch.int64, device=x.device)
+            m = stat.data_ptr()
+            run_on(x, entry, "token_logprobs",
+                   _Args(x.data_ptr(), x.stride(0), n, v, tokens.data_ptr(), tokens.dtype == torch.int64, ignore, inv_t,
+                         inv_t * _LOG2E, top_k, lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), m, m + 4 * n, ptr(top),
+                         ptr(ids), None, None, None, None, splits, ptr(part), ptr(keys)))
+        ctx.save_for_backward(x, tokens, stat, ent)
         ctx.how = (inv_t, ignore)
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(top, ids)
-        return lp, ent, lse, top, ids
+        if top_k:
+            ctx.mark_non_differentiable(top, ids)
+            return lp, ent, lse, top, ids
+        return lp, ent, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, d_lp, d_ent, d_lse, _top, _ids):
-        x, tokens, m, ls, ent = ctx.saved_tensors
+    def backward(ctx, d_lp, d_ent, d_lse, *_):
+        x, tokens, stat, ent = ctx.saved_tensors
         inv_t, ignore = ctx.how
         if not ctx.needs_input_grad[0] or (d_lp is None and d_ent is None and d_lse is None):
             return None, None, None, None, None
         if x.device.type == "cpu":
-            return _backward_torch(x, tokens, m, ls, ent, d_lp, d_ent, d_lse, inv_t, ignore), None, None, None, None
+            return _backward_torch(x, tokens, *stat, ent, d_lp, d_ent, d_lse, inv_t, ignore), None, None, None, None
         entry = native("pda_logprob_bwd")
         d_lp, d_ent, d_lse = (None if t is None else t.contiguous() for t in (d_lp, d_ent, d_lse))
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        args = _fill(_Args(), x, tokens, inv_t, ignore)
-        args.entropy, args.stat_m, args.stat_l2 = map(ptr, (ent, m, ls))
-        args.d_lp, args.d_ent, args.d_lse, args.d_logits = map(ptr, (d_lp, d_ent, d_lse, dx))
-        with on_device(x):
-            launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "token_logprobs backward")
+        n, v = x.shape
+        dx = torch.empty(n, v, dtype=x.dtype, device=x.device)
+        m = stat.data_ptr()
+        run_on(x, entry, "token_logprobs backward",
+               _Args(x.data_ptr(), x.stride(0), n, v, tokens.data_ptr(), tokens.dtype == torch.int64, ignore, inv_t,
+                     inv_t * _LOG2E, 0, None, ent.data_ptr(), None, m, m + 4 * n, None, None, ptr(d_lp), ptr(d_ent),
+                     ptr(d_lse), dx.data_ptr(), 1, None, None))
         return dx, None, None, None, None
 
 
@@ -152,8 +151,7 @@ def token_logprobs(logits, tokens, temperature=1.0, top_k=0, ignore_index=-100):
     x = logits.reshape(-1, v) if logits.dim() != 2 else logits
     if x.stride(1) != 1 and v > 1:
         x = x.contiguous()
-    lp, ent, lse, top, ids = _TokenLogprobs.apply(x, tokens.reshape(-1).contiguous(), 1.0 / temperature, top_k, ignore_index)
+    out = _TokenLogprobs.apply(x, tokens.reshape(-1).contiguous(), 1.0 / temperature, top_k, ignore_index)
     if len(lead) != 1:
-        lp, ent, lse = lp.reshape(lead), ent.reshape(lead), lse.reshape(lead)
-        top, ids = top.reshape(lead + (top_k,)), ids.reshape(lead + (top_k,))
-    return TokenLogprobs(lp, ent, lse, top if top_k else None, ids if top_k else None)
+        out = [t.reshape(lead) for t in out[:3]] + [t.reshape(lead + (top_k,)) for t in out[3:]]
+    return TokenLogprobs(*out) if top_k else TokenLogprobs(*out, None, None)

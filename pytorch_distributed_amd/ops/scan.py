@@ -9,14 +9,15 @@ import ctypes
 
 import torch
 
-from ._seq import TYPE_CODES, check_floating, check_int, launched, native, on_device, ptr, stream_of
+from ._seq import TYPE_CODES, check_floating, check_int, native, ptr, run_on
 
 GATES = ("decay", "logit")
 _vp, _i64, _int = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
 
 
 class _Args(ctypes.Structure):      # mirrors ScanArgs in csrc/scan.hip
-    _fields_ = [("x", _vp), ("gate", _vp), ("dh", _vp), ("xs", _i64 * 3), ("gs", _i64 * 3), ("ds", _i64 * 3), ("h0", _vp),
+    _fields_ = [("x", _vp), ("gate", _vp), ("dh", _vp), ("xs0", _i64), ("xs1", _i64), ("xs2", _i64),
+                ("gs0", _i64), ("gs1", _i64), ("gs2", _i64), ("ds0", _i64), ("ds1", _i64), ("ds2", _i64), ("h0", _vp),
                 ("dlast", _vp), ("lengths", _vp), ("len64", _int), ("h", _vp), ("last", _vp), ("carry", _vp),
                 ("sums", _vp), ("dx", _vp), ("dg", _vp), ("dh0", _vp), ("B", _int), ("T", _int), ("D", _int),
                 ("logit", _int), ("mix", _int), ("reverse", _int), ("chunks", _int), ("chunk_len", _int),
@@ -24,9 +25,9 @@ class _Args(ctypes.Structure):      # mirrors ScanArgs in csrc/scan.hip
 
 
 class _StepArgs(ctypes.Structure):  # mirrors ScanStepArgs
-    _fields_ = [("x", _vp), ("gate", _vp), ("state", _vp), ("state_out", _vp), ("h", _vp), ("xs", _i64 * 2),
-                ("gs", _i64 * 2), ("ss", _i64 * 2), ("os", _i64 * 2), ("B", _int), ("D", _int), ("logit", _int),
-                ("mix", _int)]
+    _fields_ = [("x", _vp), ("gate", _vp), ("state", _vp), ("state_out", _vp), ("h", _vp), ("xs0", _i64),
+                ("xs1", _i64), ("gs0", _i64), ("gs1", _i64), ("ss0", _i64), ("ss1", _i64), ("os0", _i64), ("os1", _i64),
+                ("B", _int), ("D", _int), ("logit", _int), ("mix", _int)]
 
 
 def _gate(g, logit):
@@ -96,15 +97,6 @@ def _lengths(lengths, B, T):
     return torch.full((B,), T) if lengths is None else lengths.long().clamp(0, T)
 
 
-def _fill(args, x, gate, h0, lengths, how):
-    args.x, args.gate, args.h0, args.lengths = ptr(x), ptr(gate), ptr(h0), ptr(lengths)
-    args.xs[:], args.gs[:] = x.stride(), gate.stride()
-    args.len64 = int(lengths is not None and lengths.dtype == torch.int64)
-    args.B, args.T, args.D = x.shape
-    args.logit, args.mix, args.reverse = how
-    return args
-
-
 class _LinearScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, h0, lengths, logit, mix, reverse):
@@ -117,16 +109,14 @@ class _LinearScan(torch.autograd.Function):
             entry = native("pda_scan_fwd")
             h = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
             last = torch.empty(B, D, dtype=torch.float32, device=x.device)
-            args = _fill(_Args(), x, gate, h0, lengths, how)
-            carries, args.chunks = _plan(x)
+            carries, chunks = _plan(x)
             if any(ctx.needs_input_grad):
                 carry = torch.empty(B, carries, D, dtype=torch.float32, device=x.device)
-            if args.chunks > 1:
-                sums = torch.empty(B, args.chunks, 2, D, dtype=torch.float32, device=x.device)
-                args.sums = ptr(sums)
-            args.h, args.last, args.carry = ptr(h), ptr(last), ptr(carry)
-            with on_device(x):
-                launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "linear_scan")
+            sums = torch.empty(B, chunks, 2, D, dtype=torch.float32, device=x.device) if chunks > 1 else None
+            run_on(x, entry, "linear_scan",
+                   _Args(x.data_ptr(), gate.data_ptr(), None, *x.stride(), *gate.stride(), 0, 0, 0, ptr(h0), None,
+                         ptr(lengths), lengths is not None and lengths.dtype == torch.int64, h.data_ptr(), last.data_ptr(),
+                         ptr(carry), ptr(sums), None, None, None, B, T, D, *how, chunks))
         ctx.save_for_backward(x, gate, h0, lengths, carry)
         ctx.how = how
         ctx.set_materialize_grads(False)
@@ -147,16 +137,13 @@ class _LinearScan(torch.autograd.Function):
             dlast = dlast.contiguous() if dlast is not None else None
             dx = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
             dg, dh0 = torch.empty_like(dx), torch.empty(B, D, dtype=torch.float32, device=x.device)
-            args = _fill(_Args(), x, gate, h0, lengths, ctx.how)
-            args.chunks = _plan(x)[1]
-            if args.chunks > 1:
-                sums = torch.empty(B, args.chunks, 2, D, dtype=torch.float32, device=x.device)
-                args.sums = ptr(sums)
-            args.dh, args.dlast, args.dx, args.dg, args.dh0, args.carry = map(ptr, (dh, dlast, dx, dg, dh0, carry))
-            if dh is not None:
-                args.ds[:] = dh.stride()
-            with on_device(x):
-                launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "linear_scan backward")
+            chunks = _plan(x)[1]
+            sums = torch.empty(B, chunks, 2, D, dtype=torch.float32, device=x.device) if chunks > 1 else None
+            run_on(x, entry, "linear_scan backward",
+                   _Args(x.data_ptr(), gate.data_ptr(), ptr(dh), *x.stride(), *gate.stride(),
+                         *(dh.stride() if dh is not None else (0, 0, 0)), ptr(h0), ptr(dlast), ptr(lengths),
+                         lengths is not None and lengths.dtype == torch.int64, None, None, ptr(carry), ptr(sums),
+                         dx.data_ptr(), dg.data_ptr(), dh0.data_ptr(), B, T, D, *ctx.how, chunks))
         return dx, dg, (dh0 if h0 is not None else None), None, None, None, None
 
 
@@ -213,16 +200,13 @@ def linear_scan(x, gate, h0=None, gates="decay", mix=False, reverse=False, lengt
     return (h.squeeze(2), last.squeeze(1)) if flat else (h, last)
 
 
-def _overlap(a, b):
-    """Whether the address ranges of two tensors meet."""
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in
-                                                                                zip(t.shape, t.stride())))) for t in (a, b))
-    return a0 < b1 and b0 < a1
+def _span(t):
+    """The addresses [first, behind the last) of a 2-d tensor."""
+    (n0, n1), (s0, s1) = t.shape, t.stride()
+    first = t.data_ptr()
+    return first, first + t.element_size() * ((n0 - 1) * s0 + (n1 - 1) * s1 + 1 if n0 and n1 else 0)
 
 
-@torch.no_grad()
 def linear_scan_step(x, gate, state, gates="decay", mix=False, state_out=None):
     """One step of `linear_scan` for every request of a batch: h = a state + u, returned in x's type and written in 32 bits
     to `state` itself, or to state_out, a second buffer (memory that overlaps state, x or gate otherwise than as the same view is refused).
@@ -245,18 +229,21 @@ def linear_scan_step(x, gate, state, gates="decay", mix=False, state_out=None):
         (s0, n0), (s1, n1) = sorted(zip(out.stride(), out.shape))
         if (n0 > 1 and s0 == 0) or (n1 > 1 and s1 < s0 * (n0 - 1) + 1):
             raise ValueError("the written state shares elements between requests or channels (strides %s)" % (out.stride(),))
+    first, behind = _span(out)
     for t, what in ((state, "state"), (x, "x"), (gate, "gate")):
-        if not (t.data_ptr() == out.data_ptr() and t.stride() == out.stride() and t.dtype == out.dtype) and _overlap(t, out):
+        if t is out or (t.data_ptr() == first and t.stride() == out.stride() and t.dtype == out.dtype):
+            continue
+        a, b = _span(t)
+        if a < behind and first < b:
             raise ValueError("the written state overlaps %s in memory without being the same view" % what)
     if x.device.type == "cpu":
-        h = _advance(state, x, gate, logit, mix)
-        out.copy_(h)
-        return h.to(x.dtype)
+        with torch.no_grad():
+            h = _advance(state, x, gate, logit, mix)
+            out.copy_(h)
+            return h.to(x.dtype)
     entry = native("pda_scan_step")
     h = torch.empty(B, D, dtype=x.dtype, device=x.device)
-    args = _StepArgs(ptr(x), ptr(gate), ptr(state), ptr(out), ptr(h))
-    args.xs[:], args.gs[:], args.ss[:], args.os[:] = x.stride(), gate.stride(), state.stride(), out.stride()
-    args.B, args.D, args.logit, args.mix = B, D, logit, int(bool(mix))
-    with on_device(x):
-        launched(entry(ctypes.byref(args), TYPE_CODES[x.dtype], _vp(stream_of(x))), "linear_scan_step")
+    run_on(x, entry, "linear_scan_step",
+           _StepArgs(x.data_ptr(), gate.data_ptr(), state.data_ptr(), out.data_ptr(), h.data_ptr(), *x.stride(),
+                     *gate.stride(), *state.stride(), *out.stride(), B, D, logit, bool(mix)))
     return h
