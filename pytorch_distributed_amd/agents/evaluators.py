@@ -7,13 +7,15 @@ import time
 
 import torch
 
+from ..ops.scan import linear_scan
 from ..utils.checkpoint import save_state_dict
 from ..utils.helpers import reset_experience
 from ..utils.param_store import sync_params
 
 
-def run_episodes(env, model, nepisodes, early_stop, device=torch.device("cpu"), verbose=None):
-    """Greedy rollouts; returns (total_steps, total_reward, nepisodes, nepisodes_solved)."""
+def run_episodes(env, model, nepisodes, early_stop, device=torch.device("cpu"), verbose=None, trace=None):
+    """Greedy rollouts; returns (total_steps, total_reward, nepisodes, nepisodes_solved).  trace: a list that receives
+    (reward, episode ended, value the model gave the state) per step."""
     experience = reset_experience()
     episode_steps, episode_reward = 0, 0.0
     total_steps, total_reward, done_eps, solved = 0, 0.0, 0, 0
@@ -24,7 +26,7 @@ def run_episodes(env, model, nepisodes, early_stop, device=torch.device("cpu"), 
             experience = env.reset()
             assert experience.state1 is not None
             flag_reset = False
-        action, _, _ = model.get_action(experience.state1, device=device)
+        action, _, value = model.get_action(experience.state1, device=device)
         experience = env.step(action)
         if experience.terminal1:
             solved += 1
@@ -33,6 +35,8 @@ def run_episodes(env, model, nepisodes, early_stop, device=torch.device("cpu"), 
             flag_reset = True
         episode_steps += 1
         episode_reward += experience.reward
+        if trace is not None:
+            trace.append((float(experience.reward), flag_reset, float(value)))
         if flag_reset:
             done_eps += 1
             total_steps += episode_steps
@@ -40,6 +44,20 @@ def run_episodes(env, model, nepisodes, early_stop, device=torch.device("cpu"), 
             if verbose:
                 print(verbose, done_eps)
     return total_steps, total_reward, done_eps, solved
+
+
+@torch.no_grad()
+def returns_report(trace, gamma, device=torch.device("cpu")):
+    """-> (mean discounted return of the trace's episodes, mean over its steps of the model's value minus the return that
+    followed): G_t = r_t + gamma G_{t+1}, restarted behind every episode, as ONE reversed linear recurrence over all steps.
+    An episode that was cut short counts as ended there."""
+    if not trace:
+        return 0.0, 0.0
+    rows = torch.tensor([(r, 0.0 if end else float(gamma), v) for r, end, v in trace], dtype=torch.float32).to(device)
+    returns, _ = linear_scan(rows[None, :, 0], rows[None, :, 1], reverse=True)
+    ends = [i for i, (_, end, _) in enumerate(trace) if end]
+    starts = [0] + [i + 1 for i in ends if i + 1 < len(trace)]
+    return float(returns[0, starts].mean()), float((rows[:, 2] - returns[0]).mean())
 
 
 def evaluator(process_ind, args, global_logs, evaluator_logs, env_prototype, model_prototype, global_model):
@@ -58,13 +76,18 @@ def evaluator(process_ind, args, global_logs, evaluator_logs, env_prototype, mod
 
     def evaluate_and_save():
         sync_params(local_model, global_model)
+        trace = [] if getattr(ap, "evaluate_returns", False) else None
         total_steps, total_reward, nepisodes, solved = run_episodes(
-            env, local_model, ap.evaluator_nepisodes, args.env_params.early_stop, local_device)
+            env, local_model, ap.evaluator_nepisodes, args.env_params.early_stop, local_device, trace=trace)
+        if trace is not None:
+            ret, bias = returns_report(trace, ap.gamma, torch.device(getattr(args, "device", "cpu")))
         with evaluator_logs.logger_lock.get_lock():
             evaluator_logs.total_steps.value = total_steps
             evaluator_logs.total_reward.value = total_reward
             evaluator_logs.nepisodes.value = nepisodes
             evaluator_logs.nepisodes_solved.value = solved
+            if trace is not None:
+                evaluator_logs.discounted_return.value, evaluator_logs.value_bias.value = ret, bias
             evaluator_logs.logger_lock.value = True
         print("Saving model " + args.model_name + " ...")
         save_state_dict(local_model, args.model_name)

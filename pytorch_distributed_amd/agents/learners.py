@@ -23,7 +23,10 @@ import torch
 import torch.nn as nn
 
 from ..parallel.comm import SingleComm, make_comm
+from ..ops.dropout import CounterDropout
+from ..ops.logprob import token_logprobs
 from ..utils.helpers import update_target_model
+from ..utils.options import torch_core_options
 from ..utils.param_store import AsyncParamPublisher, sync_params
 
 
@@ -47,6 +50,9 @@ class _TorchCore(object):
         self.optimizer = self.ap.optim(self.model.parameters(), lr=self.ap.lr,
                                        weight_decay=self.ap.weight_decay)
         self.model.train()
+        self.drops = [m for m in self.model.modules() if isinstance(m, CounterDropout)]
+        for m in self.drops:            # every rank draws its own masks
+            m.seed += int(getattr(self.comm, "rank", 0)) << 32
         self.step_count = 0
         self.last_losses = {}
 
@@ -85,6 +91,8 @@ class _TorchCore(object):
         keys = sorted(st)
         out = {"kind": "torch", "params": self.model.flat_params.detach().cpu().clone(),
                "target": self.target_model.flat_params.detach().cpu().clone(), "step_count": self.step_count}
+        if self.drops:
+            out["dropout_counters"] = [int(m.counter) for m in self.drops]
         if keys:
             out["exp_avg"] = torch.cat([st[k]["exp_avg"].reshape(-1).cpu() for k in keys])
             out["exp_avg_sq"] = torch.cat([st[k]["exp_avg_sq"].reshape(-1).cpu() for k in keys])
@@ -96,6 +104,8 @@ class _TorchCore(object):
             self.model.flat_params.copy_(d["params"])
             self.target_model.flat_params.copy_(d["target"])
         self.step_count = int(d["step_count"])
+        for m, c in zip(self.drops, d.get("dropout_counters", ())):     # masks go on, they do not repeat
+            m.counter.fill_(int(c))
         if "exp_avg" in d:
             off = 0
             for p in self.model.parameters():        # materialise the optimizer state, then overwrite it
@@ -118,8 +128,15 @@ class DqnTorchCore(_TorchCore):
             else:
                 next_q = self.target_model(s1).max(dim=1, keepdim=True)[0]
             target = r + g * next_q * (1 - t)
-        pred = self.model(s0).gather(1, a.long())
+        q = self.model(s0)
+        pred = q.gather(1, a.long())
         loss = self._weighted_mse(pred, target, w)
+        alpha = float(getattr(self.ap, "cql_alpha", 0.0) or 0.0)
+        if alpha != 0.0:
+            # conservative Q-learning: pushes down what the data did not do, logsumexp_a Q(s, a) - Q(s, a_taken), which is
+            # minus the log-probability of the taken action under softmax(Q)
+            taken = token_logprobs(q, a.long()[:, 0]).logprob
+            loss = loss - alpha * (w[:, 0] * taken if self.memory.enable_per else taken).mean()
         loss.backward()
         self.last_losses = {"critic_loss": loss.detach()}
         self._finish((pred.detach() - target).abs(), inds, clip_params=[list(self.model.critic.parameters())])
@@ -180,7 +197,10 @@ def _pick_compute(args, device):
 
 def make_core(kind, args, model, target_model, memory, comm, device):
     compute = _pick_compute(args, device)
-    if compute == "native":
+    only_torch = torch_core_options(args)
+    if only_torch and getattr(args, "compute", "auto") == "native":
+        raise ValueError("compute='native' does not implement %s (compute='auto' or 'torch' does)" % ", ".join(only_torch))
+    if compute == "native" and not only_torch:
         if kind == "dqn" and args.model_type == "dqn-cnn":
             from ..ops.dqn_engine import DqnNativeCore
             return DqnNativeCore(args, model, target_model, memory, comm)

@@ -35,6 +35,10 @@ def _logger_loop(process_ind, args, global_logs, actor_logs, learner_logs, evalu
                     board.add_scalar("evaluator/avg_reward", evaluator_logs.total_reward.value / n, ls)
                     board.add_scalar("evaluator/repisodes_solved", evaluator_logs.nepisodes_solved.value / n, ls)
                     board.add_scalar("evaluator/nepisodes", n, ls)
+                    if getattr(ap, "evaluate_returns", False):
+                        board.add_scalar("evaluator/avg_discounted_return", evaluator_logs.discounted_return.value, ls)
+                        if args.agent_type == "dqn":
+                            board.add_scalar("evaluator/avg_value_bias", evaluator_logs.value_bias.value, ls)
                 evaluator_logs.logger_lock.value = False
         now = time.time()
         if final or now - last_log_time > ap.logger_freq:

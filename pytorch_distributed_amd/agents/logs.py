@@ -127,4 +127,6 @@ class EvaluatorLogs(object):
         self.total_reward = mp.Value("d", 0.0)
         self.nepisodes = mp.Value("l", 0)
         self.nepisodes_solved = mp.Value("l", 0)
+        self.discounted_return = mp.Value("d", 0.0)     # (agent_params.evaluate_returns)
+        self.value_bias = mp.Value("d", 0.0)
         self.logger_lock = mp.Value("b", False)

@@ -27,6 +27,7 @@ class DdpgMlpModel(Model):
             nn.Linear(400 + self.output_dims, 300), nn.Tanh(),
             nn.Linear(300, 1),
         ))
+        self.drops = self.make_dropout(args, 2)
         self._reset()
 
     def _init_weights(self):
@@ -45,7 +46,11 @@ class DdpgMlpModel(Model):
 
     def forward_critic(self, input, action):
         qx = self.critic[0](input.float().flatten(1))
-        return self.critic[1](torch.cat((qx, action.float()), 1))
+        if self.drops is None:
+            return self.critic[1](torch.cat((qx, action.float()), 1))
+        x = torch.cat((self.drops[0](qx), action.float()), 1)
+        head = self.critic[1]
+        return head[2](self.drops[1](head[1](head[0](x))))
 
     def forward(self, input):
         action = self.forward_actor(input)

@@ -30,6 +30,7 @@ class DqnCnnModel(Model):
             nn.Linear(conv_out, 512), nn.ReLU(),
             nn.Linear(512, self.output_dims),
         ))
+        self.drops = self.make_dropout(args, 1)
         # The reference defines an orthogonal init but never calls it
         # (dqn_cnn_model.py:33), so torch's default init is what trains there.
         if getattr(args, "init", "default") == "orthogonal":
@@ -50,7 +51,11 @@ class DqnCnnModel(Model):
 
     def forward(self, input):
         x = input.float() / self.norm_val
-        return self.critic[1](self.critic[0](x).flatten(1))
+        x = self.critic[0](x).flatten(1)
+        if self.drops is None:
+            return self.critic[1](x)
+        head = self.critic[1]
+        return head[2](self.drops[0](head[1](head[0](x))))
 
     @torch.no_grad()
     def get_action(self, input, enable_per=False, eps=0.0, device=torch.device("cpu"), rng=np.random):

@@ -22,13 +22,19 @@ class DqnMlpModel(Model):
             nn.Linear(self.hidden_dims, self.hidden_dims), nn.ReLU(),
             nn.Linear(self.hidden_dims, self.output_dims),
         )
+        self.drops = self.make_dropout(args, 3)
         self._reset()
 
     def _init_weights(self):
         pass    # torch defaults, as in the reference
 
     def forward(self, input):
-        return self.critic(input.float().flatten(1) / self.norm_val)
+        x = input.float().flatten(1) / self.norm_val
+        if self.drops is None:
+            return self.critic(x)
+        for i, drop in enumerate(self.drops):
+            x = drop(self.critic[2 * i + 1](self.critic[2 * i](x)))
+        return self.critic[6](x)
 
     @torch.no_grad()
     def get_action(self, input, enable_per=False, eps=0.0, device=torch.device("cpu"), rng=np.random):

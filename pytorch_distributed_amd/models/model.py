@@ -7,6 +7,8 @@ state_dict keys and shapes are unchanged by flattening.
 import torch
 import torch.nn as nn
 
+from ..ops.dropout import CounterDropout
+
 
 class Model(nn.Module):
     def __init__(self, args, norm_val, input_dims, output_dims, action_dims):
@@ -17,6 +19,12 @@ class Model(nn.Module):
         self.action_dims = action_dims
         self._flat = None
         self._flat_grad = None
+
+    def make_dropout(self, args, sites):
+        """One dropout per site (no parameters, no state-dict entries), or nothing where args.dropout is 0."""
+        p = float(getattr(args, "dropout", 0.0) or 0.0)
+        seed = int(getattr(args, "seed", 0))
+        return nn.ModuleList([CounterDropout(p, seed=seed, site=i) for i in range(sites)]) if p != 0.0 else None
 
     def _init_weights(self):
         raise NotImplementedError("not implemented in base class")

@@ -20,6 +20,7 @@ import numpy as np
 import torch
 
 from . import hostlib
+from ..utils.options import torch_core_options
 from ..utils.param_store import sync_params
 
 
@@ -212,6 +213,8 @@ def native_learner_expected(args):
     if getattr(args, "device", "cpu") != "cuda" or getattr(args, "compute", "auto") == "torch":
         return False
     if args.model_type not in ("dqn-cnn", "ddpg-mlp"):
+        return False
+    if hasattr(args, "agent_params") and torch_core_options(args):
         return False
     if str(getattr(args, "weight_sync", "auto")) == "collective":
         return False            # an explicit request for the broadcast path implies a serving process of its own

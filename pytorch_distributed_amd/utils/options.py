@@ -278,6 +278,8 @@ class ModelParams(Params):
     def __init__(self, config=None, overrides=None):
         super().__init__(config, overrides)
         self.init = "default"           # "default" (what the reference actually runs) | "orthogonal"
+        self.dropout = 0.0              # dropped fraction behind the critic's hidden fully connected layers, in training
+                                        # passes only (ops/dropout.py; torch core; 0: as the reference)
 
 
 class AgentParams(Params):
@@ -299,6 +301,7 @@ class AgentParams(Params):
         self.max_replay_ratio = 0.0     # cap on learner updates per actor env step (0: none, as in the reference)
         self.min_replay_ratio = 0.0     # floor on the same ratio: actors wait for the learner (0: none, as in the reference)
         self.poll_interval = 5.0        # logger/evaluator wake-up period (secs; the reference hard-codes 5)
+        self.evaluate_returns = False   # evaluator / tester also report discounted returns and, for DQN, the critic's bias
         self.stop_at_eval_reward = None # end the job once an evaluation's average reward reaches this (None: run all `steps`)
         if self.agent_type == "dqn":
             self.clip_grad = np.inf
@@ -312,6 +315,8 @@ class AgentParams(Params):
             self.enable_double = False
             self.eps = 0.4
             self.eps_alpha = 7
+            self.cql_alpha = 0.0            # + this * mean(logsumexp_a Q(s, a) - Q(s, a_taken)): conservative Q-learning
+                                            # (ops/logprob.py; torch core; 0: as the reference)
         elif self.agent_type == "ddpg":
             self.clip_grad = 40.0
             self.actor_sync_freq = 400
@@ -328,6 +333,16 @@ class AgentParams(Params):
             self.ou_stationary_start = False # DDPG actors: OU noise starts at its stationary spread, not at 0 (see agents/actors.py)
             self.actor_preact_l2 = 0.0       # DDPG: + this * mean(|pre-tanh actor output|^2) in the actor loss (0: as the reference)
             self.actor_warmup_steps = 0      # DDPG: learner updates during which only the critic is trained (0: as the reference)
+
+
+def torch_core_options(args):
+    """The set options that only the torch learner core implements (the native engines' fused heads do not)."""
+    used = []
+    if float(getattr(args.agent_params, "cql_alpha", 0.0) or 0.0) != 0.0:
+        used.append("agent_params.cql_alpha")
+    if float(getattr(args.model_params, "dropout", 0.0) or 0.0) != 0.0:
+        used.append("model_params.dropout")
+    return used
 
 
 _NESTED = ("env_params", "memory_params", "model_params", "agent_params")
