@@ -31,13 +31,15 @@ __device__ __forceinline__ Gate gate_of(float g) {
     const float e = __builtin_amdgcn_exp2f(g * 1.44269504088896341f), c = __builtin_amdgcn_rcpf(1.f + e);     // a = e c
     return Gate{c <= 0.5f ? -c : e * c, c};
 }
-template <bool LOGIT>
-__device__ __forceinline__ float decayed(float h, Gate g) {         // a h
-    return LOGIT ? __builtin_fmaf(g.k, h, __builtin_bit_cast(int, g.k) < 0 ? h : 0.f) : g.k * h;
+__device__ __forceinline__ float acc_fma(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double acc_fma(double a, double b, double c) { return __builtin_fma(a, b, c); }
+template <bool LOGIT, typename Acc>
+__device__ __forceinline__ Acc decayed(Acc h, Gate g) {             // a h
+    return LOGIT ? acc_fma((Acc)g.k, h, __builtin_bit_cast(int, g.k) < 0 ? h : (Acc)0) : (Acc)g.k * h;
 }
-template <bool LOGIT, bool MIX>
-__device__ __forceinline__ float scan_step(float h, float x, Gate g) {
-    return MIX ? __builtin_fmaf(g.c, x, decayed<LOGIT>(h, g)) : decayed<LOGIT>(h, g) + x;
+template <bool LOGIT, bool MIX, typename Acc>
+__device__ __forceinline__ Acc scan_step(Acc h, float x, Gate g) {
+    return MIX ? acc_fma((Acc)g.c, (Acc)x, decayed<LOGIT>(h, g)) : decayed<LOGIT>(h, g) + (Acc)x;
 }
 __device__ __forceinline__ int scan_length(const ScanArgs& p, int b) {
     if (p.lengths == nullptr) return p.T;
@@ -61,11 +63,19 @@ __device__ __forceinline__ int scan_length(const ScanArgs& p, int b) {
 // twice.
 #define SCAN_CL 8
 // a forward tile holds a whole number of backward tiles: the forward pass leaves the state in front of each of those
-template <typename T> struct ScanFwd { static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = 32 / VEC, NT = 512; };
-template <typename T> struct ScanBwd { static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = 32 / VEC, NT = 256; };
-// fewer than 8 channels: one sequence of one channel per workgroup, of 16 waves or of one
-struct ScanRow { static constexpr int VEC = 1, CL = 1, L = 8, NT = 1024; };
-struct ScanWave { static constexpr int VEC = 1, CL = 1, L = 8, NT = 64; };
+template <typename T> struct ScanFwd {
+    typedef float Acc;
+    static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = 32 / VEC, NT = 512;
+};
+template <typename T> struct ScanBwd {
+    typedef float Acc;
+    static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = 32 / VEC, NT = 256;
+};
+// Fewer than 8 channels: one sequence of one channel per workgroup, of 16 waves or of one.  Latency is all that counts
+// there, so states and products are 64 bits wide: a constant gate such as 0.99 rounds every product the same way, which
+// left 5e-7 of 12500 discounted returns in 32 bits.
+struct ScanRow { typedef double Acc; static constexpr int VEC = 1, CL = 1, L = 8, NT = 1024; };
+struct ScanWave { typedef double Acc; static constexpr int VEC = 1, CL = 1, L = 8, NT = 64; };
 // The lanes of a wave: SW consecutive ones hold consecutive runs of steps of one group of VEC channels, so that a scan
 // over steps moves along a DPP row.
 template <typename S> struct ScanLane {
@@ -121,140 +131,6 @@ __device__ __forceinline__ Raw<T, VEC> scan_load(const T* row, long long cs, int
     }
     return r;
 }
-template <typename T, int VEC, int MODE>
-__device__ __forceinline__ void scan_store(T* row, const float (&v)[VEC], int nch) {
-    if constexpr (MODE != SCAN_ANY) {
-        vec16<T> o;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) o.e[i] = from_f32<T>(v[i]);
-        store16<MODE == SCAN_STREAM>(row, o);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-            if (i < nch) row[i] = from_f32<T>(v[i]);
-    }
-}
-// joins a later part (a, h) behind an earlier one (pa, ph): state -> a (pa state + ph) + h
-#define SCAN_JOIN(a, h, pa, ph) do { h = __builtin_fmaf(a, ph, h); a *= pa; } while (0)
-
-// Exclusive scan of the threads' parts over the workgroup, in step order (UP) or against it, applied to the state `in` in
-// front of the tile: -> the state in front of this thread's steps; `in` becomes the state behind the tile.
-// part: [waves][CL * VEC] in LDS; the caller separates two uses of one buffer by a barrier.
-template <int O, bool UP, int BANKS = 0xf>
-__device__ __forceinline__ float dpp_shift(float none, float v) {       // lane i of a row of 16 gets lane i -+ O's, or `none`
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
-                                                                 (UP ? 0x110 : 0x100) + O, 0xf, BANKS, false));
-}
-template <bool UP>
-__device__ __forceinline__ float wave_shift(float v) {                  // lane i of the wave gets lane i -+ 1's
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), UP ? 0x138 : 0x130, 0xf, 0xf, false));
-}
-template <int O, int SW, bool UP>
-__device__ __forceinline__ void scan_lanes_step(float& A, float& H) {
-    if constexpr (O < SW) {
-        constexpr int BANKS = SW == 8 && O == 4 ? (UP ? 0xa : 0x5) : 0xf;      // (the lanes of a group that have a partner)
-        float pa = dpp_shift<O, UP, BANKS>(1.f, A), ph = dpp_shift<O, UP, BANKS>(0.f, H);
-        if (SW < 16 && BANKS == 0xf) {
-            const int i = threadIdx.x & (SW - 1);
-            const bool on = UP ? i >= O : i < SW - O;
-            pa = on ? pa : 1.f;
-            ph = on ? ph : 0.f;
-        }
-        SCAN_JOIN(A, H, pa, ph);
-    }
-}
-__device__ __forceinline__ float scan_lane(float v, int lane) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
-}
-// inclusive over the SW lanes of a channel group
-template <int SW, bool UP>
-__device__ __forceinline__ void scan_lanes(float& A, float& H) {
-    static_assert(SW == 8 || SW == 16 || SW == 64, "");
-    scan_lanes_step<1, SW, UP>(A, H);
-    scan_lanes_step<2, SW, UP>(A, H);
-    scan_lanes_step<4, SW, UP>(A, H);
-    scan_lanes_step<8, SW, UP>(A, H);
-    if constexpr (SW == 64) {       // the four rows of 16
-        const int row = (threadIdx.x >> 4) & 3, at = UP ? row : 3 - row;
-        float pa = 1.f, ph = 0.f, ta = 1.f, th = 0.f;
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            const int end = UP ? 16 * k + 15 : 48 - 16 * k;
-            const float a = scan_lane(A, end), h = scan_lane(H, end);
-            th = __builtin_fmaf(a, th, h);
-            ta *= a;
-            pa = at > k ? ta : pa;
-            ph = at > k ? th : ph;
-        }
-        SCAN_JOIN(A, H, pa, ph);
-    }
-}
-template <typename S, bool UP>
-__device__ __forceinline__ void scan_across(float (&A)[S::VEC], float (&H)[S::VEC], float (&in)[S::VEC], float2* part) {
-    constexpr int NW = S::NT / 64, W = S::CL * S::VEC, SW = ScanLane<S>::SW;
-    const int wave = threadIdx.x >> 6, cl = ScanLane<S>().cl, i = threadIdx.x & (SW - 1);
-#pragma unroll
-    for (int v = 0; v < S::VEC; ++v) scan_lanes<SW, UP>(A[v], H[v]);
-    if (i == (UP ? SW - 1 : 0)) {
-#pragma unroll
-        for (int v = 0; v < S::VEC; ++v) part[wave * W + cl * S::VEC + v] = make_float2(A[v], H[v]);
-    }
-    const bool first = i == (UP ? 0 : SW - 1);
-#pragma unroll
-    for (int v = 0; v < S::VEC; ++v) {      // exclusive: the neighbour's
-        float pa, ph;
-        if constexpr (SW <= 16) {
-            pa = dpp_shift<1, UP>(1.f, A[v]);
-            ph = dpp_shift<1, UP>(0.f, H[v]);
-        } else {
-            pa = wave_shift<UP>(A[v]);
-            ph = wave_shift<UP>(H[v]);
-        }
-        A[v] = first ? 1.f : pa;
-        H[v] = first ? 0.f : ph;
-    }
-    __syncthreads();
-    float mine[S::VEC];
-#pragma unroll
-    for (int v = 0; v < S::VEC; ++v) mine[v] = in[v];
-#pragma unroll 2
-    for (int k = 0; k < NW; ++k) {          // (not unrolled further: the parts of all waves at once would take 2 VEC NW registers)
-        const int w = UP ? k : NW - 1 - k;
-#pragma unroll
-        for (int v = 0; v < S::VEC; ++v) {
-            const float2 t = part[w * W + cl * S::VEC + v];
-            if (w == wave) mine[v] = in[v];
-            in[v] = __builtin_fmaf(t.x, in[v], t.y);
-        }
-    }
-#pragma unroll
-    for (int v = 0; v < S::VEC; ++v) H[v] = __builtin_fmaf(A[v], mine[v], H[v]);
-}
-
-// the state in front of this workgroup's chunk: `in` carried over the chunks before it (UP) or behind it
-template <typename S, bool UP>
-__device__ __forceinline__ void scan_fold_chunks(const ScanArgs& p, const ScanWhere& w, float (&in)[S::VEC]) {
-    const int k0 = UP ? 0 : p.chunks - 1;
-    for (int k = k0; k != w.chunk; k += UP ? 1 : -1) {
-        const float* s = p.sums + ((long long)w.b * p.chunks + k) * 2 * p.D + w.ch0;
-#pragma unroll
-        for (int v = 0; v < S::VEC; ++v)
-            if (v < w.nch) in[v] = __builtin_fmaf(s[v], in[v], s[p.D + v]);
-    }
-}
-
-// tiles [first, last) of a chunk
-template <typename S> struct ScanTiles {
-    static constexpr int SUB = S::NT / S::CL, TILE = SUB * S::L;
-    int first, last;
-    __device__ __forceinline__ ScanTiles(const ScanArgs& p, int chunk) {
-        const int begin = min(chunk * p.chunk_len, p.T), end = min(begin + p.chunk_len, p.T);      // chunk_len: whole tiles
-        first = begin / TILE;
-        last = (end + TILE - 1) / TILE;
-        if (begin >= end) last = first;
-    }
-};
-
 // What a step that does not exist reads: it leaves the state as it is (a = 1, u = 0).
 template <typename T, int VEC, bool LOGIT>
 __device__ __forceinline__ Raw<T, VEC> scan_no_gate() {
@@ -271,72 +147,253 @@ __device__ __forceinline__ Raw<T, VEC> scan_nothing() {
     return r;
 }
 
+// The L steps from i0 of one tensor, in the recurrence's order; steps from n on read `none`.  A thread of a one-channel scan
+// whose steps are contiguous takes four 32-bit values at a time: element by element its loads would pass the L1 cache
+// (64 KB of steps in flight per workgroup) once each.
+template <typename T, typename S, int MODE>
+__device__ __forceinline__ void scan_fetch(Raw<T, S::VEC> (&r)[S::L], const T* base, long long ts, long long cs, int i0, int n,
+                                           int nch, bool reverse, const Raw<T, S::VEC>& none) {
+    constexpr int L = S::L;
+    if constexpr (S::VEC == 1 && MODE == SCAN_WIDE) {
+        if (i0 + L <= n) {
+            const T* from = base + (reverse ? n - i0 - L : i0);
+#pragma unroll
+            for (int l = 0; l < L; l += 4) {
+                uint32_t w[4];
+                __builtin_memcpy(w, from + l, 16);      // (on the 4-byte grid)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[reverse ? L - 1 - l - j : l + j].w[0] = w[j];
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+        const int i = i0 + l;
+        if (i < n && nch > 0) r[l] = scan_load<T, S::VEC, MODE != SCAN_ANY && S::VEC != 1>(base + (reverse ? n - 1 - i : i) * ts, cs, nch);
+        else r[l] = none;
+    }
+}
+template <typename T, int VEC, int MODE>
+__device__ __forceinline__ void scan_store(T* row, const float (&v)[VEC], int nch) {
+    if constexpr (MODE != SCAN_ANY && VEC != 1) {
+        vec16<T> o;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o.e[i] = from_f32<T>(v[i]);
+        store16<MODE == SCAN_STREAM>(row, o);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < nch) row[i] = from_f32<T>(v[i]);
+    }
+}
+// joins a later part (a, h) behind an earlier one (pa, ph): state -> a (pa state + ph) + h
+#define SCAN_JOIN(a, h, pa, ph) do { h = acc_fma(a, ph, h); a *= pa; } while (0)
+template <typename Acc> struct alignas(2 * sizeof(Acc)) Part { Acc a, h; };
+
+template <int CTRL, int BANKS>
+__device__ __forceinline__ float dpp_move(float none, float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
+                                                                 CTRL, 0xf, BANKS, false));
+}
+template <int CTRL, int BANKS>
+__device__ __forceinline__ double dpp_move(double none, double v) {
+    const uint2 n = __builtin_bit_cast(uint2, none), w = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_update_dpp(n.x, w.x, CTRL, 0xf, BANKS, false),
+                                                 __builtin_amdgcn_update_dpp(n.y, w.y, CTRL, 0xf, BANKS, false)));
+}
+template <int O, bool UP, int BANKS = 0xf, typename Acc>
+__device__ __forceinline__ Acc dpp_shift(Acc none, Acc v) {             // lane i of a row of 16 gets lane i -+ O's, or `none`
+    return dpp_move<(UP ? 0x110 : 0x100) + O, BANKS>(none, v);
+}
+template <bool UP, typename Acc>
+__device__ __forceinline__ Acc wave_shift(Acc v) {                      // lane i of the wave gets lane i -+ 1's
+    return dpp_move<UP ? 0x138 : 0x130, 0xf>((Acc)0, v);
+}
+__device__ __forceinline__ float scan_lane(float v, int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+__device__ __forceinline__ double scan_lane(double v, int lane) {
+    const uint2 w = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_readlane(w.x, lane), __builtin_amdgcn_readlane(w.y, lane)));
+}
+template <int O, int SW, bool UP, typename Acc>
+__device__ __forceinline__ void scan_lanes_step(Acc& A, Acc& H) {
+    if constexpr (O < SW) {
+        constexpr int BANKS = SW == 8 && O == 4 ? (UP ? 0xa : 0x5) : 0xf;      // (the lanes of a group that have a partner)
+        Acc pa = dpp_shift<O, UP, BANKS>((Acc)1, A), ph = dpp_shift<O, UP, BANKS>((Acc)0, H);
+        if (SW < 16 && BANKS == 0xf) {
+            const int i = threadIdx.x & (SW - 1);
+            const bool on = UP ? i >= O : i < SW - O;
+            pa = on ? pa : (Acc)1;
+            ph = on ? ph : (Acc)0;
+        }
+        SCAN_JOIN(A, H, pa, ph);
+    }
+}
+// inclusive over the SW lanes of a channel group
+template <int SW, bool UP, typename Acc>
+__device__ __forceinline__ void scan_lanes(Acc& A, Acc& H) {
+    static_assert(SW == 8 || SW == 16 || SW == 64, "");
+    scan_lanes_step<1, SW, UP>(A, H);
+    scan_lanes_step<2, SW, UP>(A, H);
+    scan_lanes_step<4, SW, UP>(A, H);
+    scan_lanes_step<8, SW, UP>(A, H);
+    if constexpr (SW == 64) {       // the four rows of 16
+        const int row = (threadIdx.x >> 4) & 3, at = UP ? row : 3 - row;
+        Acc pa = 1, ph = 0, ta = 1, th = 0;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const int end = UP ? 16 * k + 15 : 48 - 16 * k;
+            const Acc a = scan_lane(A, end), h = scan_lane(H, end);
+            th = acc_fma(a, th, h);
+            ta *= a;
+            pa = at > k ? ta : pa;
+            ph = at > k ? th : ph;
+        }
+        SCAN_JOIN(A, H, pa, ph);
+    }
+}
+// Exclusive scan of the threads' parts over the workgroup, in step order (UP) or against it, applied to the state `in` in
+// front of the tile: H becomes the state in front of this thread's steps, `in` the state behind the tile.
+// part: [waves][CL * VEC] in LDS; the caller separates two uses of one buffer by a barrier.
+template <typename S, bool UP, typename Acc>
+__device__ __forceinline__ void scan_across(Acc (&A)[S::VEC], Acc (&H)[S::VEC], Acc (&in)[S::VEC], Part<Acc>* part) {
+    constexpr int NW = S::NT / 64, W = S::CL * S::VEC, SW = ScanLane<S>::SW;
+    const int wave = threadIdx.x >> 6, cl = ScanLane<S>().cl, i = threadIdx.x & (SW - 1);
+#pragma unroll
+    for (int v = 0; v < S::VEC; ++v) scan_lanes<SW, UP>(A[v], H[v]);
+    if (i == (UP ? SW - 1 : 0)) {
+#pragma unroll
+        for (int v = 0; v < S::VEC; ++v) part[wave * W + cl * S::VEC + v] = Part<Acc>{A[v], H[v]};
+    }
+    const bool first = i == (UP ? 0 : SW - 1);
+#pragma unroll
+    for (int v = 0; v < S::VEC; ++v) {      // exclusive: the neighbour's
+        Acc pa, ph;
+        if constexpr (SW <= 16) {
+            pa = dpp_shift<1, UP>((Acc)1, A[v]);
+            ph = dpp_shift<1, UP>((Acc)0, H[v]);
+        } else {
+            pa = wave_shift<UP>(A[v]);
+            ph = wave_shift<UP>(H[v]);
+        }
+        A[v] = first ? (Acc)1 : pa;
+        H[v] = first ? (Acc)0 : ph;
+    }
+    __syncthreads();
+    Acc mine[S::VEC];
+#pragma unroll
+    for (int v = 0; v < S::VEC; ++v) mine[v] = in[v];
+#pragma unroll 2
+    for (int k = 0; k < NW; ++k) {          // (not unrolled further: the parts of all waves at once would take 2 VEC NW registers)
+        const int w = UP ? k : NW - 1 - k;
+#pragma unroll
+        for (int v = 0; v < S::VEC; ++v) {
+            const Part<Acc> t = part[w * W + cl * S::VEC + v];
+            if (w == wave) mine[v] = in[v];
+            in[v] = acc_fma(t.a, in[v], t.h);
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < S::VEC; ++v) H[v] = acc_fma(A[v], mine[v], H[v]);
+}
+
+// `in` carried over the chunks in front of this workgroup's (UP) or behind it: one chunk per thread row and round
+template <typename S, bool UP, typename Acc>
+__device__ __forceinline__ void scan_fold_chunks(const ScanArgs& p, const ScanWhere& w, Acc (&in)[S::VEC], Part<Acc>* part) {
+    constexpr int SUB = S::NT / S::CL;
+    const int count = UP ? w.chunk : p.chunks - 1 - w.chunk, sub = ScanLane<S>().sub;
+    for (int base = 0; base < count; base += SUB) {
+        const int j = base + (UP ? sub : SUB - 1 - sub), k = UP ? j : p.chunks - 1 - j;
+        Acc A[S::VEC], H[S::VEC];
+#pragma unroll
+        for (int v = 0; v < S::VEC; ++v) {
+            const bool on = j < count && v < w.nch;
+            const float* s = p.sums + ((long long)w.b * p.chunks + (on ? k : 0)) * 2 * p.D + (on ? w.ch0 + v : 0);
+            A[v] = on ? s[0] : 1.f;
+            H[v] = on ? s[p.D] : 0.f;
+        }
+        scan_across<S, UP>(A, H, in, part);
+        __syncthreads();        // (part is used again)
+    }
+}
+
+// tiles [first, last) of a chunk
+template <typename S> struct ScanTiles {
+    static constexpr int SUB = S::NT / S::CL, TILE = SUB * S::L;
+    int first, last;
+    __device__ __forceinline__ ScanTiles(const ScanArgs& p, int chunk) {
+        const int begin = min(chunk * p.chunk_len, p.T), end = min(begin + p.chunk_len, p.T);      // chunk_len: whole tiles
+        first = begin / TILE;
+        last = (end + TILE - 1) / TILE;
+        if (begin >= end) last = first;
+    }
+};
+
+// The next tile's loads are issued as soon as this tile's registers are free, over the joins and the stores.  (A second set
+// of registers, loaded a whole tile ahead, took 65 us instead of 54 at 8 x 2048 x 2048 bf16: 240 registers a thread.)
 template <typename T, typename S, bool LOGIT, bool MIX, int MODE>
 __global__ __launch_bounds__(S::NT) void scan_fwd_kernel(ScanArgs p) {
+    typedef typename S::Acc Acc;
     constexpr int VEC = S::VEC, L = S::L, TILE = ScanTiles<S>::TILE;
-    __shared__ float2 part[2][S::NT / 64 * S::CL * VEC];
+    __shared__ Part<Acc> part[2][S::NT / 64 * S::CL * VEC];
     const ScanWhere w = scan_where<S>(p);
     const ScanTiles<S> tl(p, w.chunk);
     const int sub = ScanLane<S>().sub;
     const T* x = (const T*)p.x + w.b * p.xs[0] + w.ch0 * p.xs[2];
     const T* g = (const T*)p.gate + w.b * p.gs[0] + w.ch0 * p.gs[2];
     T* out = (T*)p.h + (long long)w.b * p.T * p.D + w.ch0;
-    Raw<T, VEC> xr[L], gr[L];
-    auto fetch = [&](int tile) {
-#pragma unroll
-        for (int l = 0; l < L; ++l) {
-            const int i = tile * TILE + sub * L + l;
-            if (i < w.n && w.nch > 0) {
-                const long long t = p.reverse ? w.n - 1 - i : i;
-                xr[l] = scan_load<T, VEC, MODE != SCAN_ANY>(x + t * p.xs[1], p.xs[2], w.nch);
-                gr[l] = scan_load<T, VEC, MODE != SCAN_ANY>(g + t * p.gs[1], p.gs[2], w.nch);
-            } else {
-                xr[l] = scan_nothing<T, VEC>();
-                gr[l] = scan_no_gate<T, VEC, LOGIT>();
-            }
-        }
+    struct Set { Raw<T, VEC> x[L], g[L]; };
+    auto fetch = [&](Set& s, int tile) {
+        const int i0 = tile * TILE + sub * L;
+        scan_fetch<T, S, MODE>(s.x, x, p.xs[1], p.xs[2], i0, w.n, w.nch, p.reverse, scan_nothing<T, VEC>());
+        scan_fetch<T, S, MODE>(s.g, g, p.gs[1], p.gs[2], i0, w.n, w.nch, p.reverse, scan_no_gate<T, VEC, LOGIT>());
     };
-    fetch(tl.first);
-    float in[VEC];
+    Set s;
+    fetch(s, tl.first);
+    Acc in[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) in[v] = p.h0 && v < w.nch ? p.h0[(long long)w.b * p.D + w.ch0 + v] : 0.f;
-    scan_fold_chunks<S, true>(p, w, in);
+    scan_fold_chunks<S, true>(p, w, in, part[0]);
     for (int tile = tl.first; tile < tl.last; ++tile) {
         const int i0 = tile * TILE + sub * L;
-        float A[L][VEC], H[L][VEC];
-        float start[VEC];       // the state in front of this thread's steps
+        Acc A[L][VEC], H[L][VEC], a[VEC], h[VEC];
+        const bool some = tile * TILE < w.n;
+        if (some) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) start[v] = 0.f;
-        if (tile * TILE < w.n) {
-            float a[VEC], h[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) { a[v] = 1.f; h[v] = 0.f; }
+            for (int v = 0; v < VEC; ++v) { a[v] = 1; h[v] = 0; }
 #pragma unroll
             for (int l = 0; l < L; ++l) {
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    const Gate ga = gate_of<LOGIT>(gr[l].get(v));
-                    h[v] = scan_step<LOGIT, MIX>(h[v], xr[l].get(v), ga);
+                    const Gate ga = gate_of<LOGIT>(s.g[l].get(v));
+                    h[v] = scan_step<LOGIT, MIX>(h[v], s.x[l].get(v), ga);
                     a[v] = decayed<LOGIT>(a[v], ga);
                     A[l][v] = a[v];
                     H[l][v] = h[v];
                 }
             }
-            if (tile + 1 < tl.last) fetch(tile + 1);            // in flight over the scan and the stores
+            if (tile + 1 < tl.last) fetch(s, tile + 1);
             scan_across<S, true>(a, h, in, part[tile & 1]);     // (two buffers: one barrier per tile)
+        } else {
 #pragma unroll
-            for (int l = 0; l < L; ++l) {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) H[l][v] = __builtin_fmaf(A[l][v], h[v], H[l][v]);
-            }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) start[v] = h[v];
+            for (int v = 0; v < VEC; ++v) h[v] = 0;
         }
         if (p.carry != nullptr && i0 % p.carry_len == 0 && i0 < p.T) {
             float* c = p.carry + ((long long)w.b * p.carries + i0 / p.carry_len) * p.D + w.ch0;
 #pragma unroll
             for (int v = 0; v < VEC; ++v)
-                if (v < w.nch) c[v] = start[v];
+                if (v < w.nch) c[v] = (float)h[v];
+        }
+        if constexpr (VEC == 1 && MODE == SCAN_WIDE) {
+            if (i0 + L <= w.n && p.D == 1) {
+                float o[L];
+#pragma unroll
+                for (int l = 0; l < L; ++l) o[p.reverse ? L - 1 - l : l] = (float)acc_fma(A[l][0], h[0], H[l][0]);
+                __builtin_memcpy(out + (p.reverse ? w.n - i0 - L : i0), o, sizeof(o));      // (32-bit elements)
+                continue;
+            }
         }
 #pragma unroll
         for (int l = 0; l < L; ++l) {
@@ -346,21 +403,22 @@ __global__ __launch_bounds__(S::NT) void scan_fwd_kernel(ScanArgs p) {
             const long long t = on && p.reverse ? w.n - 1 - i : i;
             float o[VEC];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) o[v] = on ? H[l][v] : 0.f;
+            for (int v = 0; v < VEC; ++v) o[v] = on ? (float)acc_fma(A[l][v], h[v], H[l][v]) : 0.f;
             scan_store<T, VEC, MODE>(out + t * p.D, o, w.nch);
         }
     }
     if (w.chunk == p.chunks - 1 && sub == 0) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v)
-            if (v < w.nch) p.last[(long long)w.b * p.D + w.ch0 + v] = in[v];
+            if (v < w.nch) p.last[(long long)w.b * p.D + w.ch0 + v] = (float)in[v];
     }
 }
 
 template <typename T, typename S, bool LOGIT, bool MIX, int MODE>
 __global__ __launch_bounds__(S::NT) void scan_bwd_kernel(ScanArgs p) {
+    typedef typename S::Acc Acc;
     constexpr int VEC = S::VEC, L = S::L, TILE = ScanTiles<S>::TILE;
-    __shared__ float2 part[2][S::NT / 64 * S::CL * VEC];
+    __shared__ Part<Acc> part[2][S::NT / 64 * S::CL * VEC];
     const ScanWhere w = scan_where<S>(p);
     const ScanTiles<S> tl(p, w.chunk);
     const int sub = ScanLane<S>().sub;
@@ -368,51 +426,42 @@ __global__ __launch_bounds__(S::NT) void scan_bwd_kernel(ScanArgs p) {
     const T* g = (const T*)p.gate + w.b * p.gs[0] + w.ch0 * p.gs[2];
     const T* dh = (const T*)p.dh + w.b * p.ds[0] + w.ch0 * p.ds[2];
     const long long base = (long long)w.b * p.T * p.D + w.ch0;
-    Raw<T, VEC> xr[L], gr[L], dr[L];
-    float hin[VEC];
-    auto fetch = [&](int tile) {
-#pragma unroll
-        for (int l = 0; l < L; ++l) {
-            const int i = tile * TILE + sub * L + l;
-            const bool on = i < w.n && w.nch > 0;
-            const long long t = p.reverse ? w.n - 1 - i : i;
-            if (on) {
-                gr[l] = scan_load<T, VEC, MODE != SCAN_ANY>(g + t * p.gs[1], p.gs[2], w.nch);
-                xr[l] = scan_load<T, VEC, MODE != SCAN_ANY>(x + t * p.xs[1], p.xs[2], w.nch);
-            } else {
-                gr[l] = scan_no_gate<T, VEC, LOGIT>();
-                xr[l] = scan_nothing<T, VEC>();
-            }
-            if (on && p.dh != nullptr) dr[l] = scan_load<T, VEC, MODE != SCAN_ANY>(dh + t * p.ds[1], p.ds[2], w.nch);
-            else dr[l] = scan_nothing<T, VEC>();
-        }
+    struct Set { Raw<T, VEC> x[L], g[L], d[L]; float hin[VEC]; };
+    auto fetch = [&](Set& s, int tile) {
+        const int i0 = tile * TILE + sub * L, n = w.n;
+        scan_fetch<T, S, MODE>(s.g, g, p.gs[1], p.gs[2], i0, n, w.nch, p.reverse, scan_no_gate<T, VEC, LOGIT>());
+        scan_fetch<T, S, MODE>(s.x, x, p.xs[1], p.xs[2], i0, n, w.nch, p.reverse, scan_nothing<T, VEC>());
+        scan_fetch<T, S, MODE>(s.d, dh, p.ds[1], p.ds[2], i0, p.dh != nullptr ? n : 0, w.nch, p.reverse, scan_nothing<T, VEC>());
 #pragma unroll
         for (int v = 0; v < VEC; ++v)
-            hin[v] = v < w.nch ? p.carry[((long long)w.b * p.carries + tile) * p.D + w.ch0 + v] : 0.f;
+            s.hin[v] = v < w.nch ? p.carry[((long long)w.b * p.carries + tile) * p.D + w.ch0 + v] : 0.f;
     };
-    if (tl.last > tl.first) fetch(tl.last - 1);
-    float rin[VEC];
+    Set s;
+    if (tl.last > tl.first) fetch(s, tl.last - 1);
+    Acc rin[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) rin[v] = p.dlast && v < w.nch ? p.dlast[(long long)w.b * p.D + w.ch0 + v] : 0.f;
-    scan_fold_chunks<S, false>(p, w, rin);
+    scan_fold_chunks<S, false>(p, w, rin, part[0]);
     for (int tile = tl.last - 1; tile >= tl.first; --tile) {
         const int i0 = tile * TILE + sub * L;
         // per step: G = q + P r_in, dx = G c or G, dgate = G wt
-        float P[L][VEC], q[L][VEC], wt[L][VEC], cc[L][VEC], a[VEC], h[VEC];
+        Acc P[L][VEC], q[L][VEC], a[VEC], h[VEC];
+        float wt[L][VEC], cc[L][VEC];
         const bool some = tile * TILE < w.n;
         if (some) {
             Gate ga[L][VEC];
+            Acc hin[VEC];
             // the tile's states again: wt = the state in front of step l (- x), first relative to the thread's start
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) { a[v] = 1.f; h[v] = 0.f; }
+            for (int v = 0; v < VEC; ++v) { a[v] = 1; h[v] = 0; hin[v] = s.hin[v]; }
 #pragma unroll
             for (int l = 0; l < L; ++l) {
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    const float xv = xr[l].get(v);
-                    ga[l][v] = gate_of<LOGIT>(gr[l].get(v));
+                    const float xv = s.x[l].get(v);
+                    ga[l][v] = gate_of<LOGIT>(s.g[l].get(v));
                     P[l][v] = a[v];
-                    wt[l][v] = MIX ? h[v] - xv : h[v];
+                    q[l][v] = MIX ? h[v] - (Acc)xv : h[v];
                     h[v] = scan_step<LOGIT, MIX>(h[v], xv, ga[l][v]);
                     a[v] = decayed<LOGIT>(a[v], ga[l][v]);
                 }
@@ -422,26 +471,26 @@ __global__ __launch_bounds__(S::NT) void scan_bwd_kernel(ScanArgs p) {
             for (int l = 0; l < L; ++l) {
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    wt[l][v] = __builtin_fmaf(P[l][v], h[v], wt[l][v]);
+                    wt[l][v] = (float)acc_fma(P[l][v], h[v], q[l][v]);
                     if (LOGIT) wt[l][v] *= decayed<LOGIT>(ga[l][v].c, ga[l][v]);      // a c
                 }
             }
             // r = a G, carried from later steps to earlier ones; P and q relative to the thread's end
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) { a[v] = 1.f; h[v] = 0.f; }
+            for (int v = 0; v < VEC; ++v) { a[v] = 1; h[v] = 0; }
 #pragma unroll
             for (int l = L - 1; l >= 0; --l) {
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
                     P[l][v] = a[v];
-                    q[l][v] = h[v] + dr[l].get(v);
+                    q[l][v] = h[v] + (Acc)s.d[l].get(v);
                     h[v] = decayed<LOGIT>(q[l][v], ga[l][v]);
                     a[v] = decayed<LOGIT>(a[v], ga[l][v]);
                     if (MIX) cc[l][v] = ga[l][v].c;
                 }
             }
         }
-        if (tile > tl.first) fetch(tile - 1);       // in flight over the second scan and the stores
+        if (tile > tl.first) fetch(s, tile - 1);
         if (some) scan_across<S, false>(a, h, rin, part[1]);
 #pragma unroll
         for (int l = 0; l < L; ++l) {
@@ -452,7 +501,7 @@ __global__ __launch_bounds__(S::NT) void scan_bwd_kernel(ScanArgs p) {
             float ox[VEC], og[VEC];
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const float G = __builtin_fmaf(P[l][v], h[v], q[l][v]);
+                const float G = (float)acc_fma(P[l][v], h[v], q[l][v]);
                 ox[v] = on ? (MIX ? G * cc[l][v] : G) : 0.f;
                 og[v] = on ? G * wt[l][v] : 0.f;
             }
@@ -463,7 +512,7 @@ __global__ __launch_bounds__(S::NT) void scan_bwd_kernel(ScanArgs p) {
     if (w.chunk == 0 && sub == 0) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v)
-            if (v < w.nch) p.dh0[(long long)w.b * p.D + w.ch0 + v] = rin[v];
+            if (v < w.nch) p.dh0[(long long)w.b * p.D + w.ch0 + v] = (float)rin[v];
     }
 }
 
@@ -471,8 +520,9 @@ __global__ __launch_bounds__(S::NT) void scan_bwd_kernel(ScanArgs p) {
 // A thread walks a run of its own through the chunk; the runs are joined once.
 template <typename T, typename S, bool LOGIT, bool MIX, bool UP, int MODE>
 __global__ __launch_bounds__(S::NT) void scan_sum_kernel(ScanArgs p) {
+    typedef typename S::Acc Acc;
     constexpr int VEC = S::VEC, SUB = ScanTiles<S>::SUB, U = 4;
-    __shared__ float2 part[S::NT / 64 * S::CL * VEC];
+    __shared__ Part<Acc> part[S::NT / 64 * S::CL * VEC];
     const ScanWhere w = scan_where<S>(p);
     const int sub = ScanLane<S>().sub;
     const T* v1 = UP ? (const T*)p.x : (const T*)p.dh;
@@ -481,18 +531,18 @@ __global__ __launch_bounds__(S::NT) void scan_sum_kernel(ScanArgs p) {
     v1 += w.b * s0 + w.ch0 * s2;
     const int begin = min(w.chunk * p.chunk_len, p.T), end = min(min(begin + p.chunk_len, p.T), w.n), run = (max(end - begin, 0) + SUB - 1) / SUB;
     const int i0 = begin + sub * run, i1 = w.nch > 0 ? min(i0 + run, end) : i0;
-    float a[VEC], h[VEC];
+    Acc a[VEC], h[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) { a[v] = 1.f; h[v] = 0.f; }
+    for (int v = 0; v < VEC; ++v) { a[v] = 1; h[v] = 0; }
     for (int k = i0; k < i1; k += U) {
         Raw<T, VEC> gr[U], vr[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int j = min(k + u, i1 - 1), i = UP ? j : i0 + (i1 - 1 - j);
             const long long t = p.reverse ? w.n - 1 - i : i;
-            gr[u] = scan_load<T, VEC, MODE != SCAN_ANY>(g + t * p.gs[1], p.gs[2], w.nch);
+            gr[u] = scan_load<T, VEC, MODE != SCAN_ANY && VEC != 1>(g + t * p.gs[1], p.gs[2], w.nch);
             if (UP || p.dh != nullptr) {
-                vr[u] = scan_load<T, VEC, MODE != SCAN_ANY>(v1 + t * s1, s2, w.nch);
+                vr[u] = scan_load<T, VEC, MODE != SCAN_ANY && VEC != 1>(v1 + t * s1, s2, w.nch);
             } else {
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) vr[u].put(v, from_f32<T>(0.f));
@@ -505,8 +555,8 @@ __global__ __launch_bounds__(S::NT) void scan_sum_kernel(ScanArgs p) {
             for (int v = 0; v < VEC; ++v) {
                 const Gate ga = gate_of<LOGIT>(gr[u].get(v));
                 const float xv = vr[u].get(v);
-                const float hv = UP ? scan_step<LOGIT, MIX>(h[v], xv, ga) : decayed<LOGIT>(h[v] + xv, ga);
-                const float av = decayed<LOGIT>(a[v], ga);
+                const Acc hv = UP ? scan_step<LOGIT, MIX>(h[v], xv, ga) : decayed<LOGIT>(h[v] + (Acc)xv, ga);
+                const Acc av = decayed<LOGIT>(a[v], ga);
                 h[v] = on ? hv : h[v];
                 a[v] = on ? av : a[v];
             }
@@ -518,29 +568,33 @@ __global__ __launch_bounds__(S::NT) void scan_sum_kernel(ScanArgs p) {
     for (int v = 0; v < VEC; ++v) scan_lanes<SW, UP>(a[v], h[v]);
     if (li == (UP ? SW - 1 : 0)) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) part[wave * S::CL * VEC + cl * VEC + v] = make_float2(a[v], h[v]);
+        for (int v = 0; v < VEC; ++v) part[wave * S::CL * VEC + cl * VEC + v] = Part<Acc>{a[v], h[v]};
     }
     __syncthreads();
     if (wave == 0 && li == 0) {
         float* out = p.sums + ((long long)w.b * p.chunks + w.chunk) * 2 * p.D + w.ch0;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            float ta = 1.f, th = 0.f;
+            Acc ta = 1, th = 0;
 #pragma unroll
             for (int k = 0; k < S::NT / 64; ++k) {
-                const float2 t = part[(UP ? k : S::NT / 64 - 1 - k) * S::CL * VEC + cl * VEC + v];
-                th = __builtin_fmaf(t.x, th, t.y);
-                ta *= t.x;
+                const Part<Acc> t = part[(UP ? k : S::NT / 64 - 1 - k) * S::CL * VEC + cl * VEC + v];
+                th = acc_fma(t.a, th, t.h);
+                ta *= t.a;
             }
-            if (v < w.nch) { out[v] = ta; out[p.D + v] = th; }
+            if (v < w.nch) { out[v] = (float)ta; out[p.D + v] = (float)th; }
         }
     }
 }
 
-#ifndef SCAN_CHUNK_TILES
-#define SCAN_CHUNK_TILES 4
-#endif
 // How a problem is cut (the forward and the backward pass of one call agree on it: a function of the sizes alone).
+//
+// Chunks: where the slabs are fewer than the 256 CUs and there are at least SCAN_CHUNK_TILES tiles, the steps are cut into
+// as many chunks as give every CU one workgroup; with fewer tiles the second reading and its launch take longer than the
+// tiles that they save.  (Chunks taken in turns that fit the memory-side cache, so that the second reading finds them
+// there: 323 us against 326 us at 1 x 65521 x 512 fp32 with gradient, not worth it.)
+#define SCAN_CHUNK_TILES 8
+#define SCAN_ROUND 256
 struct ScanPlan { int kind, slabs, chunks, chunk_len, carry_len, carries; };
 #define SCAN_KIND_SLAB 0
 #define SCAN_KIND_ROW 1
@@ -551,15 +605,12 @@ static void scan_cut(ScanPlan& k, long long groups, int T) {
     const int tile = ScanTiles<F>::TILE, tiles = (T + tile - 1) / tile;
     k.carry_len = ScanTiles<B>::TILE;
     k.carries = (T + k.carry_len - 1) / k.carry_len;
-    // chunks of at least SCAN_CHUNK_TILES tiles where the workgroups would leave CUs idle: below that the second reading
-    // and its launch take longer than the tiles that they save
-    long long want = groups > 0 && groups < 256 ? (512 + groups - 1) / groups : 1;
-    if (want > tiles / SCAN_CHUNK_TILES) want = tiles / SCAN_CHUNK_TILES;
-    if (want > 64) want = 64;
-    if (want < 1) want = 1;
-    const int per = (int)((tiles + want - 1) / want);
-    k.chunks = per > 0 ? (tiles + per - 1) / per : 1;
-    k.chunk_len = per > 0 ? per * tile : tile;
+    k.chunks = 1;
+    k.chunk_len = (tiles > 0 ? tiles : 1) * tile;
+    if (groups <= 0 || groups >= SCAN_ROUND || tiles < SCAN_CHUNK_TILES) return;
+    const int want = (int)(SCAN_ROUND / groups < tiles ? SCAN_ROUND / groups : tiles), per = (tiles + want - 1) / want;
+    k.chunks = (tiles + per - 1) / per;
+    k.chunk_len = per * tile;
 }
 static ScanPlan scan_plan(int B, int T, int D, int dtype) {
     ScanPlan k;
@@ -614,6 +665,11 @@ static void scan_dispatch(const ScanArgs& p, const ScanPlan& k, bool backward, h
     constexpr int VEC = 16 / sizeof(T);
     const bool wide = scan_wide(p.x, p.xs, p.D, VEC) && scan_wide(p.gate, p.gs, p.D, VEC) &&
                       (!backward || p.dh == nullptr || scan_wide(p.dh, p.ds, p.D, VEC));
+    if constexpr (sizeof(T) == 4) {     // one channel whose steps are contiguous
+        const bool steps = p.D == 1 && p.xs[1] == 1 && p.gs[1] == 1 && (!backward || p.dh == nullptr || p.ds[1] == 1);
+        if (steps && k.kind == SCAN_KIND_ROW) return scan_forms<T, ScanRow, ScanRow, SCAN_WIDE>(p, k, backward, stream);
+        if (steps && k.kind == SCAN_KIND_WAVE) return scan_forms<T, ScanWave, ScanWave, SCAN_WIDE>(p, k, backward, stream);
+    }
     if (k.kind == SCAN_KIND_ROW) scan_forms<T, ScanRow, ScanRow, SCAN_ANY>(p, k, backward, stream);
     else if (k.kind == SCAN_KIND_WAVE) scan_forms<T, ScanWave, ScanWave, SCAN_ANY>(p, k, backward, stream);
     else if (!wide) scan_forms<T, ScanFwd<T>, ScanBwd<T>, SCAN_ANY>(p, k, backward, stream);
