@@ -260,7 +260,7 @@ __device__ __forceinline__ void scan_lanes(Acc& A, Acc& H) {
 template <typename S, bool UP, typename Acc>
 __device__ __forceinline__ void scan_across(Acc (&A)[S::VEC], Acc (&H)[S::VEC], Acc (&in)[S::VEC], Part<Acc>* part) {
     constexpr int NW = S::NT / 64, W = S::CL * S::VEC, SW = ScanLane<S>::SW;
-    const int wave = threadIdx.x >> 6, cl = ScanLane<S>().cl, i = threadIdx.x & (SW - 1);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), cl = ScanLane<S>().cl, i = threadIdx.x & (SW - 1);
 #pragma unroll
     for (int v = 0; v < S::VEC; ++v) scan_lanes<SW, UP>(A[v], H[v]);
     if (i == (UP ? SW - 1 : 0)) {
@@ -283,17 +283,16 @@ __device__ __forceinline__ void scan_across(Acc (&A)[S::VEC], Acc (&H)[S::VEC], 
     }
     __syncthreads();
     Acc mine[S::VEC];
+    const Part<Acc>* t = part + (UP ? 0 : (NW - 1) * W) + cl * S::VEC;
+    const int at = UP ? wave : NW - 1 - wave;
 #pragma unroll
-    for (int v = 0; v < S::VEC; ++v) mine[v] = in[v];
-#pragma unroll 2
-    for (int k = 0; k < NW; ++k) {          // (not unrolled further: the parts of all waves at once would take 2 VEC NW registers)
-        const int w = UP ? k : NW - 1 - k;
+    for (int k = 0; k < NW; ++k, t += UP ? W : -W) {
+        if (k == at) {
 #pragma unroll
-        for (int v = 0; v < S::VEC; ++v) {
-            const Part<Acc> t = part[w * W + cl * S::VEC + v];
-            if (w == wave) mine[v] = in[v];
-            in[v] = acc_fma(t.a, in[v], t.h);
+            for (int v = 0; v < S::VEC; ++v) mine[v] = in[v];
         }
+#pragma unroll
+        for (int v = 0; v < S::VEC; ++v) in[v] = acc_fma(t[v].a, in[v], t[v].h);
     }
 #pragma unroll
     for (int v = 0; v < S::VEC; ++v) H[v] = acc_fma(A[v], mine[v], H[v]);

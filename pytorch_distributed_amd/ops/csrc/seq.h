@@ -35,6 +35,7 @@ template <typename T> struct alignas(16) vec16 { T e[16 / sizeof(T)]; };
 // pushes them out of it: the gradient of 4096 x 32000 bf16 logits (262 MB) took 107 us through the caches and 78 us past
 // them, and the next forward pass over the same logits 65 and 48 us.  Outputs that do fit stay for whoever reads them next.
 typedef __attribute__((ext_vector_type(4))) int seq_i32x4;
+typedef __attribute__((ext_vector_type(4))) unsigned seq_u32x4;
 #define SEQ_STREAM_BYTES (96ll << 20)
 template <bool STREAM, typename T>
 __device__ __forceinline__ void store16(T* to, const vec16<T>& v) {

@@ -90,6 +90,31 @@ def test_logprob_sizes(dev, dt, n, v, k):
 
 
 @pytest.mark.gpu
+def test_logprob_large_tensors_equal_their_parts():
+    x = torch.empty(2048, 32000, dtype=torch.bfloat16, device="cuda").normal_() * 2       # 131 MB: stores past the caches
+    tok = torch.randint(0, 32000, (2048,), device="cuda")
+
+    def run(sl):
+        leaf = x[sl].detach().requires_grad_()
+        o = token_logprobs(leaf, tok[sl])
+        d, = torch.autograd.grad(o.logprob.sum() + o.entropy.sum(), leaf)
+        return o.logprob.detach(), o.entropy.detach(), d
+    whole = run(slice(None))
+    for a, b in zip(whole, run(slice(512, 1536))):      # (no split of the rows in either)
+        assert torch.equal(a[512:1536], b)
+
+
+@pytest.mark.gpu
+def test_dropout_large_tensors():
+    n = 50 * (1 << 20) + 16         # 100 MB: stores past the caches
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    y = dropout(x, 0.5, 9, counter_at(2, "cuda"), residual=x)
+    for at in (0, 1 << 20, n - 4096):
+        want = 1 + 2 * oracle.keep_mask(range(at, at + 4096), 0.5, 9, 2, 0).astype(np.float64)
+        assert np.array_equal(np64(y[at:at + 4096]), want)
+
+
+@pytest.mark.gpu
 @on_types
 @pytest.mark.parametrize("n,v,k", [(1, 131072, 20), (61, 50257, 5), (2, 200003, 32), (300, 3001, 0), (1030, 2048, 4)])
 def test_logprob_large(dt, n, v, k):
@@ -287,6 +312,40 @@ def test_scan_long(dt, gates, mix, reverse, b, t, d):
     check_scan(x, g, rand((b, d), torch.float32, "cuda", 7), None, gates, mix, reverse)
     n = torch.tensor([t - 1, 0, t // 3][:b], device="cuda")
     check_scan(x, g, rand((b, d), torch.float32, "cuda", 7), n, gates, mix, reverse)
+
+
+@on_devices
+@on_types
+@pytest.mark.parametrize("d", [5, 33, 64])
+def test_scan_every_form(dev, dt, d):
+    """Each combination of gates, mixing and direction, whole tiles and parts, with and without 16-byte accesses."""
+    for gates in ("decay", "logit"):
+        for mix in (False, True):
+            for reverse in (False, True):
+                x, g = scan_inputs((2, 70, d), dt, dev, gates, seed=d)
+                check_scan(x, g, rand((2, d), torch.float32, dev, 7), torch.tensor([70, 64], device=dev), gates, mix, reverse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gates,mix,reverse", FORMS)
+def test_scan_large_tensors_equal_their_parts(gates, mix, reverse):
+    """Above 96 MB stores go past the caches; 48 sequences at once and 8 at a time are the same arithmetic."""
+    shape = (48, 520, 2048)
+    x = torch.empty(shape, dtype=torch.bfloat16, device="cuda").normal_()
+    g = torch.empty(shape, dtype=torch.bfloat16, device="cuda").normal_() * 1.5 + 2
+    if gates == "decay":
+        g = torch.sigmoid(g)
+    n = torch.arange(48, device="cuda") * 11 + 3
+    dh = torch.empty_like(x).normal_()
+
+    def run(sl):
+        leaves = [t[sl].detach().requires_grad_() for t in (x, g)]
+        h, last = linear_scan(*leaves, gates=gates, mix=mix, reverse=reverse, lengths=n[sl])
+        return (h.detach(), last.detach()) + torch.autograd.grad((h, last), leaves, (dh[sl], torch.ones_like(last)))
+    whole = run(slice(None))
+    for i in range(0, 48, 8):
+        for a, b in zip(whole, run(slice(i, i + 8))):
+            assert torch.equal(a[i:i + 8], b)
 
 
 @on_devices
