@@ -42,6 +42,10 @@ __device__ __forceinline__ uint64_t lp_key(float x, int i) {
     return ((uint64_t)b << 32) | (uint32_t)~i;
 }
 __device__ __forceinline__ int lp_key_index(uint64_t k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ float lp_key_value(uint64_t k) {         // (0 for -0: its log-probability is the same)
+    const uint32_t b = (uint32_t)(k >> 32);
+    return __builtin_bit_cast(float, (b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
+}
 __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -126,25 +130,26 @@ __device__ __forceinline__ float lp_log2_sum(LpStat st) {
     if (st.m == INFINITY || st.s != st.s) return __builtin_nanf("");
     return st.s == 0.f ? 0.f : __builtin_amdgcn_logf(st.s);
 }
+// The given token's logit, NaN for a token outside the vocabulary.  (Its load is issued with the row's, not behind its sums.)
 template <typename T>
-__device__ __forceinline__ void lp_finish_row(const LogprobArgs& p, long long row, long long tok, LpStat st, const LpRow& q) {
-    const T* x = (const T*)p.logits + row * p.ld;
-    p.logprob[row] = tok >= 0 && tok < p.vocab ? q.logp(to_f32(x[tok]), p.inv_t) : __builtin_nanf("");
+__device__ __forceinline__ float lp_given(const LogprobArgs& p, const T* x, long long tok) {
+    return tok >= 0 && tok < p.vocab ? to_f32(x[tok]) : __builtin_nanf("");
+}
+__device__ __forceinline__ void lp_finish_row(const LogprobArgs& p, long long row, float xt, LpStat st, const LpRow& q) {
+    p.logprob[row] = xt == xt ? q.logp(xt, p.inv_t) : xt;
     p.entropy[row] = q.empty ? 0.f : (q.l2 - st.u / st.s) * LP_LN2;
     p.lse[row] = q.empty ? -INFINITY : q.near ? (q.r + q.l2) * LP_LN2 : __builtin_fmaf(q.m, p.inv_t, q.l2 * LP_LN2);
     p.stat_m[row] = st.m;
     p.stat_l2[row] = q.l2;
 }
-template <typename T>
 __device__ __forceinline__ void lp_put_alternative(const LogprobArgs& p, long long row, int k, uint64_t key, const LpRow& q) {
-    const int id = lp_key_index(key);
-    p.top_id[row * p.top_k + k] = id;
-    p.top_lp[row * p.top_k + k] = q.logp(to_f32(((const T*)p.logits + row * p.ld)[id]), p.inv_t);
+    p.top_id[row * p.top_k + k] = lp_key_index(key);
+    p.top_lp[row * p.top_k + k] = q.logp(lp_key_value(key), p.inv_t);
 }
 
 // Rows that the running statistics cannot take: nothing but -inf, NaN, +inf, or |m c| beyond LP_NEAR.  Whole workgroup, two walks and one more for each alternative.
 template <typename T>
-__device__ __forceinline__ void lp_walk_row(const LogprobArgs& p, long long row, long long tok, LpStat* part, uint64_t* best) {
+__device__ __forceinline__ void lp_walk_row(const LogprobArgs& p, long long row, float xt, LpStat* part, uint64_t* best) {
     const T* x = (const T*)p.logits + row * p.ld;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     float m = -INFINITY, bad = 0.f;
@@ -174,7 +179,7 @@ __device__ __forceinline__ void lp_walk_row(const LogprobArgs& p, long long row,
     __syncthreads();
     const LpStat st{m, (part[0].s + part[1].s) + (part[2].s + part[3].s), (part[0].u + part[1].u) + (part[2].u + part[3].u)};
     LpRow q(m, lp_log2_sum(st), p.c, true);
-    if (tid == 0) lp_finish_row<T>(p, row, tok, st, q);
+    if (tid == 0) lp_finish_row(p, row, xt, st, q);
     uint64_t last = ~0ull;
     for (int k = 0; k < p.top_k; ++k) {
         uint64_t b = 0;
@@ -188,7 +193,7 @@ __device__ __forceinline__ void lp_walk_row(const LogprobArgs& p, long long row,
         __syncthreads();
         last = best[0];
         for (int w = 1; w < 4; ++w) last = best[w] > last ? best[w] : last;
-        if (tid == 0) lp_put_alternative<T>(p, row, k, last, q);
+        if (tid == 0) lp_put_alternative(p, row, k, last, q);
     }
     __syncthreads();
 }
@@ -219,6 +224,7 @@ __global__ __launch_bounds__(256) void logprob_short_kernel(LogprobArgs p) {
         const long long tok = on ? lp_token(p, row) : p.ignore;
         const bool live = on && tok != p.ignore;
         const T* x = (const T*)p.logits + (live ? row : 0) * p.ld;
+        const float xt = live && l == 0 ? lp_given(p, x, tok) : 0.f;
         float xs[E], m = -INFINITY, bad = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -241,7 +247,7 @@ __global__ __launch_bounds__(256) void logprob_short_kernel(LogprobArgs p) {
         const LpStat st{m, s, u};
         const LpRow q(m, lp_log2_sum(st), p.c, true);
         if (l == 0 && on) {
-            if (live) lp_finish_row<T>(p, row, tok, st, q);
+            if (live) lp_finish_row(p, row, xt, st, q);
             else lp_ignored_row(p, row);
         }
         uint64_t last = ~0ull;
@@ -259,7 +265,7 @@ __global__ __launch_bounds__(256) void logprob_short_kernel(LogprobArgs p) {
                 b = t > b ? t : b;
             }
             last = b;
-            if (l == 0 && live) lp_put_alternative<T>(p, row, k, last, q);
+            if (l == 0 && live) lp_put_alternative(p, row, k, last, q);
         }
     }
 }
@@ -274,6 +280,12 @@ __device__ __forceinline__ uint64_t lp_next_lane(uint64_t v) {      // lane i ge
     const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)v, 0x138, 0xf, 0xf, false);
     return ((uint64_t)hi << 32) | lo;
 }
+// LDS written by some lanes of a wave and read by others
+__device__ __forceinline__ void lp_wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+#define LP_FIRST 128       // keys that a wave's first batch may hold in LDS
 // A wave's best keys, sorted over its lanes, and what a value has to reach (`strict`: to exceed) to come among them.
 struct LpList {
     uint64_t key; float lim; bool strict, full;
@@ -303,11 +315,30 @@ struct LpList {
             const uint64_t up = lp_next_lane(key);
             key = lane < pos ? key : (lane == pos ? q : up);
         }
+        settle(k);
+    }
+    // the first values at once: n <= LP_FIRST keys in `from` (this wave's LDS), ordered by counting what is above each
+    __device__ __forceinline__ void fill(const uint64_t* from, uint64_t* sorted, int n, int k) {
+        const int lane = threadIdx.x & 63;
+        lp_wave_fence();
+        const uint64_t q0 = lane < n ? from[lane] : 0, q1 = lane + 64 < n ? from[lane + 64] : 0;
+        int a0 = 0, a1 = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const uint64_t o = from[j];
+            a0 += o > q0 ? 1 : 0;
+            a1 += o > q1 ? 1 : 0;
+        }
+        if (q0 != 0 && a0 < 64) sorted[a0] = q0;
+        if (q1 != 0 && a1 < 64) sorted[a1] = q1;
+        lp_wave_fence();
+        key = lane < n ? sorted[lane] : 0;
+        settle(k);
+    }
+    __device__ __forceinline__ void settle(int k) {
         const uint64_t kth = lp_lane(key, k - 1);
         if (kth == 0) return;
-        uint32_t b = (uint32_t)(kth >> 32);
-        b = (b & 0x80000000u) ? (b & 0x7fffffffu) : ~b;
-        const float v = __builtin_bit_cast(float, b);
+        const float v = lp_key_value(kth);
         if (!full || v > lim) { lim = v; strict = false; }      // equal values of this batch may have lower indices
         full = true;
     }
@@ -317,12 +348,19 @@ struct LpList {
 // Each thread keeps running statistics, shifted once per 32 or 16 values.  The alternatives: each wave keeps its best keys
 // sorted over its lanes.  A value is looked at again only if it passes the wave's k-th best, which the first batch sets to
 // the k-th largest of the lanes' maxima; a wave of n values then inserts about k (2 + ln(n / 2048)) of them, each by a
-// ballot and a shift by one lane.
-template <typename T, bool TOP>
+// ballot and a shift by one lane.  FILL: the first batch, which is all that a wave of a split row mostly sees, is ordered
+// at once instead (1 row of 131072 bf16, 20 alternatives: 11.4 -> 10.0 us; in the loop over a whole row the same code costs
+// more than it saves: 4096 rows 248 -> 277 us).
+//
+// 4096 x 32000 bf16 without alternatives: 48.4 us, 5.4 TB/s of the 5.4 to 5.7 that a copy or a sum of 256 MB reaches here.
+// 4096 x 131072 bf16 with 8 alternatives: 248 us, 4.3 TB/s (a sum of 1 GB: 4.0 to 4.4).  Split rows are bound by the
+// latency of the chain of loads, joins and the second launch: 1 x 131072 10.0 + 4.6 us.  (Workgroups of 1024 threads with a
+// shared limit, so that fewer parts are joined: 16 to 32 us.)
+template <typename T, bool TOP, bool FILL>
 __global__ __launch_bounds__(256, 4) void logprob_long_kernel(LogprobArgs p) {
     constexpr int VEC = 16 / sizeof(T), U = 2, NX = U * VEC;
     __shared__ LpStat part[4];
-    __shared__ uint64_t keys[4 * LP_MAX_TOP];
+    __shared__ uint64_t keys[4 * LP_MAX_TOP], firsts[FILL ? 4 : 1][LP_FIRST], sorted[FILL ? 4 : 1][64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const float c = p.c;
     const long long units = p.rows * p.splits;
@@ -335,6 +373,7 @@ __global__ __launch_bounds__(256, 4) void logprob_long_kernel(LogprobArgs p) {
             continue;
         }
         const T* x = (const T*)p.logits + row * p.ld;
+        const float xt = p.splits == 1 && tid == 0 ? lp_given(p, x, tok) : 0.f;
         // head: tokens in front of the first 16-byte boundary; behind the vectors the tail
         const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T), p.vocab);
         const int nvec = (p.vocab - head) / VEC, tail = (p.vocab - head) - nvec * VEC;
@@ -372,14 +411,26 @@ __global__ __launch_bounds__(256, 4) void logprob_long_kernel(LogprobArgs p) {
 #pragma unroll
             for (int i = 0; i < NX; ++i)
                 if (list.passes(xs[i]) && b + (i / VEC) * 256 + tid < v1) mask |= 1u << i;
+            bool first = FILL && b == v0;
+            int count = 0;              // of the first batch's keys
             for (uint64_t todo = __ballot(mask != 0); todo; todo = __ballot(mask != 0)) {
                 const int slot = __builtin_ctz(mask | 0x80000000u);
                 mask &= mask - 1;
                 float v = xs[0];
 #pragma unroll
                 for (int i = 1; i < NX; ++i) v = slot == i ? xs[i] : v;
-                list.insert(todo, lp_key(v, head + (b + (slot / VEC) * 256 + tid) * VEC + slot % VEC), p.top_k);
+                const uint64_t key = lp_key(v, head + (b + (slot / VEC) * 256 + tid) * VEC + slot % VEC);
+                const int more = __builtin_popcountll(todo);
+                if (first && count + more <= LP_FIRST) {
+                    if (todo >> lane & 1) firsts[wave][count + __builtin_popcountll(todo & ((1ull << lane) - 1))] = key;
+                    count += more;
+                    continue;
+                }
+                if (FILL && first) list.fill(firsts[wave], sorted[wave], count, p.top_k);
+                first = false;
+                list.insert(todo, key, p.top_k);
             }
+            if (FILL && first) list.fill(firsts[wave], sorted[wave], count, p.top_k);
         };
         vec16<T> even[U], odd[U];
         fetch(even, v0);
@@ -414,16 +465,16 @@ __global__ __launch_bounds__(256, 4) void logprob_long_kernel(LogprobArgs p) {
             __syncthreads();
             lp_rank(keys, 4 * p.top_k, p.top_k, [&](int k, uint64_t key) { p.part_top[unit * p.top_k + k] = key; });
         } else if (!lp_ordinary(st, c)) {
-            lp_walk_row<T>(p, row, tok, part, keys);
+            lp_walk_row<T>(p, row, xt, part, keys);
         } else {
             const LpRow q(st.m, lp_log2_sum(st), c, false);
-            if (tid == 0) lp_finish_row<T>(p, row, tok, st, q);
-            lp_rank(keys, 4 * p.top_k, p.top_k, [&](int k, uint64_t key) { lp_put_alternative<T>(p, row, k, key, q); });
+            if (tid == 0) lp_finish_row(p, row, xt, st, q);
+            lp_rank(keys, 4 * p.top_k, p.top_k, [&](int k, uint64_t key) { lp_put_alternative(p, row, k, key, q); });
         }
         __syncthreads();            // part[] and keys[] are reused by the next unit
     }
 }
-// Joins the splits of a row.  Of their sorted lists only keys that reach the k-th largest of the lists' first ceil(k /
+// Joins the splits of a row, one per lane.  Of their sorted lists only keys that reach the k-th largest of the lists' first ceil(k /
 // splits) entries can be among the best: mostly k and a few more.
 #define LP_JOIN_KEYS 1024
 template <typename T>
@@ -438,32 +489,37 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs p) {
         if (tid == 0) lp_ignored_row(p, row);
         return;
     }
-    LpStat st{-INFINITY, 0.f, 0.f};         // (every wave merges all splits: no exchange between waves)
-    for (int s = lane; s < p.splits; s += 64) {
-        const float* q = p.part_stat + (row * p.splits + s) * 4;
-        st = lp_merge(st, LpStat{q[0], q[1], q[2]}, p.c);
-    }
-    st = lp_across<64>(st, p.c);
+    // everything this row needs is asked for at once
+    const float xt = tid == 0 ? lp_given(p, (const T*)p.logits + row * p.ld, tok) : 0.f;
+    float4 own{-INFINITY, 0.f, 0.f, 0.f};       // (every wave merges all splits: no exchange between waves)
+    if (lane < p.splits) own = reinterpret_cast<const float4*>(p.part_stat)[row * p.splits + lane];
+    constexpr int PER = LP_JOIN_KEYS / 256;
+    uint64_t mine[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) mine[j] = tid + j * 256 < n ? p.part_top[row * n + tid + j * 256] : 0;
+    if (tid == 0) { count = 0; limit = 0; }
+    const LpStat st = lp_across<64>(LpStat{own.x, own.y, own.z}, p.c);
     if (!lp_ordinary(st, p.c)) {
-        lp_walk_row<T>(p, row, tok, part, keys);
+        lp_walk_row<T>(p, row, xt, part, keys);
         return;
     }
     const LpRow q(st.m, lp_log2_sum(st), p.c, false);
-    if (tid == 0) lp_finish_row<T>(p, row, tok, st, q);
+    if (tid == 0) lp_finish_row(p, row, xt, st, q);
     if (k == 0) return;
-    const unsigned long long* top = p.part_top + row * n;
     const int deep = (k + p.splits - 1) / p.splits, nh = deep * p.splits;       // k <= nh < k + splits <= 96
-    if (tid == 0) { count = 0; limit = 0; }
-    if (tid < nh) heads[tid] = top[(tid / deep) * k + tid % deep];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = tid + j * 256, split = i / k, at = i - split * k;
+        if (i < n && at < deep) heads[split * deep + at] = mine[j];
+    }
     __syncthreads();
     lp_rank(heads, nh, k, [&](int r, uint64_t key) { if (r == k - 1) limit = key; });
     __syncthreads();
-    for (int i = tid; i < n; i += 256) {
-        const uint64_t key = top[i];
-        if (key != 0 && key >= limit) keys[atomicAdd(&count, 1)] = key;     // (any order: lp_rank sorts)
-    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        if (mine[j] != 0 && mine[j] >= limit) keys[atomicAdd(&count, 1)] = mine[j];     // (any order: lp_rank sorts)
     __syncthreads();
-    lp_rank(keys, count, k, [&](int r, uint64_t key) { lp_put_alternative<T>(p, row, r, key, q); });
+    lp_rank(keys, count, k, [&](int r, uint64_t key) { lp_put_alternative(p, row, r, key, q); });
 }
 
 // ---- gradient ----------------------------------------------------------------------------------------------------------
@@ -608,8 +664,9 @@ static void lp_launch(const LogprobArgs& p, bool backward, hipStream_t stream) {
     } else {
         const long long units = p.rows * p.splits;
         const dim3 grid((unsigned)(units < 1048576 ? units : 1048576)), block(256);
-        if (p.top_k > 0) hipLaunchKernelGGL((logprob_long_kernel<T, true>), grid, block, 0, stream, p);
-        else hipLaunchKernelGGL((logprob_long_kernel<T, false>), grid, block, 0, stream, p);
+        if (p.top_k > 0 && p.splits > 1) hipLaunchKernelGGL((logprob_long_kernel<T, true, true>), grid, block, 0, stream, p);
+        else if (p.top_k > 0) hipLaunchKernelGGL((logprob_long_kernel<T, true, false>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((logprob_long_kernel<T, false, false>), grid, block, 0, stream, p);
         if (p.splits > 1) hipLaunchKernelGGL(logprob_join_kernel<T>, dim3((unsigned)p.rows), dim3(256), 0, stream, p);
     }
 }

@@ -129,7 +129,7 @@ def token_logprobs(logits, tokens, temperature=1.0, top_k=0, ignore_index=-100):
     tokens        [...] int32 or int64: the tokens (actions) whose log-probabilities are wanted.  `ignore_index` marks a
                   padded row: its logits are not read, its outputs and gradient are 0, its alternatives' tokens -1.  Any
                   other value outside [0, V) gives NaN, in the log-probability and in the row's gradient.
-    temperature   > 0;  top_k: 0 .. min(32, V) alternatives, best first, the lower token of equals first
+    temperature   2^-126 .. 2^126;  top_k: 0 .. min(32, V) alternatives, best first, the lower token of equals first
 
     logprob, entropy and logsumexp (float32, shaped as tokens) are differentiable with respect to logits;
     top_logprobs (float32) and top_tokens (int64), [..., top_k], are not, and are None for top_k = 0.
@@ -140,8 +140,8 @@ def token_logprobs(logits, tokens, temperature=1.0, top_k=0, ignore_index=-100):
         raise ValueError("logits must have a last dimension of at least one token, not shape %s" % (tuple(logits.shape),))
     check_int(tokens, "tokens", logits.shape[:-1], logits.device)
     temperature = float(temperature)
-    if not (temperature > 0.0 and math.isfinite(temperature)):
-        raise ValueError("temperature must be positive and finite, not %r" % temperature)
+    if not 2.0 ** -126 <= temperature <= 2.0 ** 126:        # (1 / T is a 32-bit factor)
+        raise ValueError("temperature must be in [2^-126, 2^126], not %r" % temperature)
     v = logits.shape[-1]
     if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= min(MAX_TOP, v):
         raise ValueError("top_k must be an int in [0, %d], not %r" % (min(MAX_TOP, v), top_k))

@@ -240,6 +240,22 @@ def test_logprob_refusals(dev):
             token_logprobs(*args, **kw)
 
 
+@on_devices
+@pytest.mark.parametrize("v", (8, 2000))
+def test_logprob_temperatures_at_the_borders(dev, v):
+    """1 / T is a 32-bit factor: temperatures whose 1 / T or log2(e) / T leaves the normal numbers are refused."""
+    x, t = torch.zeros(2, v, device=dev), torch.tensor([3, 4], device=dev)
+    x[:, 3] = 1.0
+    for T in (2.0 ** -127, 1e-39, 2.0 ** 127, 1e300):
+        with pytest.raises(ValueError):
+            token_logprobs(x, t, temperature=T)
+    hot = token_logprobs(x, t, temperature=2.0 ** 126).logprob
+    assert (hot + math.log(v)).abs().max() < 4 * 2.0 ** -24 * math.log(v)       # a log and one product, each within an ulp
+    cold = token_logprobs(x, t, temperature=2.0 ** -126)
+    assert cold.logprob[0] == 0 and cold.logsumexp[0] == 2.0 ** 126 and cold.entropy.tolist() == [0.0, 0.0]
+    assert abs(float(cold.logprob[1]) / 2.0 ** 126 + 1) < 4 * 2.0 ** -24        # (two roundings, c's and that of c ln 2)
+
+
 # ---- linear recurrence ---------------------------------------------------------------------------------------------
 def check_scan(x, gate, h0=None, lengths=None, gates="decay", mix=False, reverse=False, seed=0, grads=True):
     dt = x.dtype
