@@ -33,6 +33,15 @@ def native(name):
         raise RuntimeError("%s on a GPU needs the HIP library: %s" % (name, native_error()))
 
 
+def differentiable_once(backward):
+    """torch's once_differentiable, without its wrapper (5 us a call) where no graph of the gradient is asked for."""
+    with_graph = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (with_graph if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
 def ptr(t):
     return t.data_ptr() if t is not None else None
 

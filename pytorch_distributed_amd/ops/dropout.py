@@ -11,7 +11,7 @@ import ctypes
 import torch
 import torch.nn as nn
 
-from ._seq import check_floating, native, ptr, run_on
+from ._seq import check_floating, differentiable_once, native, ptr, run_on
 
 _M64 = (1 << 64) - 1
 _GOLDEN = 0x9E3779B97F4A7C15
@@ -81,7 +81,7 @@ class _Dropout(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @differentiable_once
     def backward(ctx, dy):
         used, = ctx.saved_tensors
         dx = _run(dy.contiguous(), None, *ctx.how, used, None) if ctx.needs_input_grad[0] else None
@@ -115,7 +115,7 @@ def dropout(x, p, seed, counter, site=0, residual=None):
         if not isinstance(residual, torch.Tensor) or residual.dtype != x.dtype or residual.shape != x.shape or \
                 residual.device != x.device:
             raise ValueError("residual must have x's shape, type and device")
-    return _Dropout.apply(x, residual, p, seed, site, counter.detach().reshape(1))
+    return _Dropout.apply(x, residual, p, seed, site, counter if counter.dim() == 1 else counter.reshape(1))
 
 
 class CounterDropout(nn.Module):

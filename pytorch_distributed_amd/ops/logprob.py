@@ -11,7 +11,7 @@ from collections import namedtuple
 
 import torch
 
-from ._seq import check_floating, check_int, native, ptr, run_on
+from ._seq import check_floating, check_int, differentiable_once, native, ptr, run_on
 
 MAX_TOP = 32        # csrc/logprob.hip LP_MAX_TOP
 TokenLogprobs = namedtuple("TokenLogprobs", "logprob, entropy, logsumexp, top_logprobs, top_tokens")
@@ -101,7 +101,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return lp, ent, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @differentiable_once
     def backward(ctx, d_lp, d_ent, d_lse, *_):
         x, tokens, stat, ent = ctx.saved_tensors
         inv_t, ignore = ctx.how

@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from ._seq import TYPE_CODES, check_floating, check_int, native, ptr, run_on
+from ._seq import TYPE_CODES, check_floating, check_int, differentiable_once, native, ptr, run_on
 
 GATES = ("decay", "logit")
 _vp, _i64, _int = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
@@ -123,7 +123,7 @@ class _LinearScan(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @differentiable_once
     def backward(ctx, dh, dlast):
         x, gate, h0, lengths, carry = ctx.saved_tensors
         none = (None,) * 7

@@ -707,6 +707,21 @@ def policy_data(dev, b=3, t=21, d=24, v=37):
 
 
 @on_devices
+@pytest.mark.parametrize("op", ("logprob", "scan", "dropout"))
+def test_gradients_are_not_differentiated_again(dev, op):
+    """A graph of the gradient may be asked for (as a larger graph does); going through it is refused, not wrong."""
+    x = rand((3, 4, 8), torch.float32, dev, 0).requires_grad_()
+    y = {"logprob": lambda: token_logprobs(x, torch.zeros(3, 4, dtype=torch.int64, device=dev)).logprob,
+         "scan": lambda: linear_scan(x, torch.full_like(x, 0.5))[0],
+         "dropout": lambda: dropout(x, 0.25, 1, counter_at(0, dev))}[op]()
+    plain, = torch.autograd.grad(y.square().sum(), x, retain_graph=True)
+    d, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    assert torch.equal(d, plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.sum(), x)
+
+
+@on_devices
 def test_recurrent_policy_step(dev):
     x, wg, wo, tokens, adv, n = policy_data(dev)
     leaves = [q.clone().requires_grad_() for q in (x, wg, wo)]
