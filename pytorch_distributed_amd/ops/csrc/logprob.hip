@@ -18,7 +18,7 @@ struct LogprobArgs {
     const void* tokens; int tok64; long long ignore;
     float inv_t, c; int top_k;                          // 1 / T, log2(e) / T
     float* logprob; float* entropy; float* lse;         // [rows]
-    float* stat_m; float* stat_l2;                      // [rows]: m, log2 s, for the backward pass
+    float* stat_m; float* stat_l2;                      // [rows]: m, log2 s, for the backward pass (null: none follows)
     float* top_lp; long long* top_id;                   // [rows][top_k]
     // backward
     const float* d_lp; const float* d_ent; const float* d_lse;  // [rows], any may be null
@@ -105,7 +105,7 @@ __device__ __forceinline__ LpStat lp_across(LpStat st, float c) {
 
 __device__ __forceinline__ void lp_ignored_row(const LogprobArgs& p, long long row) {
     p.logprob[row] = 0.f; p.entropy[row] = 0.f; p.lse[row] = 0.f;
-    p.stat_m[row] = 0.f; p.stat_l2[row] = 0.f;
+    if (p.stat_m) { p.stat_m[row] = 0.f; p.stat_l2[row] = 0.f; }
     for (int k = 0; k < p.top_k; ++k) { p.top_lp[row * p.top_k + k] = 0.f; p.top_id[row * p.top_k + k] = -1; }
 }
 
@@ -139,8 +139,7 @@ __device__ __forceinline__ void lp_finish_row(const LogprobArgs& p, long long ro
     p.logprob[row] = xt == xt ? q.logp(xt, p.inv_t) : xt;
     p.entropy[row] = q.empty ? 0.f : (q.l2 - st.u / st.s) * LP_LN2;
     p.lse[row] = q.empty ? -INFINITY : q.near ? (q.r + q.l2) * LP_LN2 : __builtin_fmaf(q.m, p.inv_t, q.l2 * LP_LN2);
-    p.stat_m[row] = st.m;
-    p.stat_l2[row] = q.l2;
+    if (p.stat_m) { p.stat_m[row] = st.m; p.stat_l2[row] = q.l2; }
 }
 __device__ __forceinline__ void lp_put_alternative(const LogprobArgs& p, long long row, int k, uint64_t key, const LpRow& q) {
     p.top_id[row * p.top_k + k] = lp_key_index(key);
@@ -674,7 +673,9 @@ static int lp_run(const LogprobArgs* args, int dtype, bool backward, hipStream_t
     const LogprobArgs p = *args;
     if (!lp_ok(p) || dtype < SEQ_F32 || dtype > SEQ_F16) return SEQ_REFUSED;
     if (p.rows == 0) return 0;
-    if (!backward) {
+    if (backward) {
+        if (p.stat_m == nullptr || p.stat_l2 == nullptr) return SEQ_REFUSED;
+    } else {
         if (p.splits != lp_splits(p.rows, p.vocab, p.top_k)) return SEQ_REFUSED;
         if (p.splits > 1 && (p.part_stat == nullptr || (p.top_k > 0 && p.part_top == nullptr))) return SEQ_REFUSED;
     }

@@ -74,7 +74,7 @@ def _run(x, residual, p, seed, site, counter, used):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, site, counter):
-        used = torch.empty_like(counter) if any(ctx.needs_input_grad) else None
+        used = torch.empty_like(counter)
         y = _run(x.contiguous(), residual.contiguous() if residual is not None else None, p, seed, site, counter, used)
         ctx.save_for_backward(used)
         ctx.how = (p, seed, site)
@@ -115,7 +115,10 @@ def dropout(x, p, seed, counter, site=0, residual=None):
         if not isinstance(residual, torch.Tensor) or residual.dtype != x.dtype or residual.shape != x.shape or \
                 residual.device != x.device:
             raise ValueError("residual must have x's shape, type and device")
-    return _Dropout.apply(x, residual, p, seed, site, counter if counter.dim() == 1 else counter.reshape(1))
+    counter = counter if counter.dim() == 1 else counter.reshape(1)
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _Dropout.apply(x, residual, p, seed, site, counter)
+    return _run(x.contiguous(), residual.contiguous() if residual is not None else None, p, seed, site, counter, None)
 
 
 class CounterDropout(nn.Module):

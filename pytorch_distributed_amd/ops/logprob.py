@@ -68,30 +68,35 @@ def _backward_torch(x, tokens, m, ls, ent, d_lp, d_ent, d_lse, inv_t, ignore):
     return torch.where(off[:, None], torch.zeros_like(g), g).to(x.dtype)
 
 
+def _forward(x, tokens, inv_t, top_k, ignore, keep):
+    """-> (logprob, entropy, logsumexp, top_logprobs, top_tokens, stat); stat: what a backward pass needs, if `keep`"""
+    n, v = x.shape
+    if x.device.type == "cpu":
+        lp, ent, lse, m, ls, top, ids = _forward_torch(x, tokens, inv_t, top_k, ignore)
+        return lp, ent, lse, top, ids, torch.stack([m, ls])
+    entry = native("pda_logprob")
+    kw = {"dtype": torch.float32, "device": x.device}
+    lp, ent, lse = torch.empty(n, **kw), torch.empty(n, **kw), torch.empty(n, **kw)
+    stat = torch.empty(2, n, **kw) if keep else None
+    top = torch.empty(n, top_k, **kw) if top_k else None
+    ids = torch.empty(n, top_k, dtype=torch.int64, device=x.device) if top_k else None
+    splits, part, m = 1, 0, stat.data_ptr() if keep else 0
+    if v > 1024:
+        splits = native("pda_logprob_splits")(_i64(n), v, top_k)
+    if splits > 1:      # long rows in parts, joined by a second launch: four floats and top_k keys for each part
+        work = torch.empty(n * splits * (2 + top_k), dtype=torch.int64, device=x.device)
+        part = work.data_ptr()
+    run_on(x, entry, "token_logprobs",
+           _Args(x.data_ptr(), x.stride(0), n, v, tokens.data_ptr(), tokens.dtype == torch.int64, ignore, inv_t,
+                 inv_t * _LOG2E, top_k, lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), m, m + 4 * n if keep else 0, ptr(top),
+                 ptr(ids), None, None, None, None, splits, part, part + 16 * n * splits))
+    return lp, ent, lse, top, ids, stat
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tokens, inv_t, top_k, ignore):
-        n = x.shape[0]
-        if x.device.type == "cpu":
-            lp, ent, lse, m, ls, top, ids = _forward_torch(x, tokens, inv_t, top_k, ignore)
-            stat = torch.stack([m, ls])
-        else:
-            entry = native("pda_logprob")
-            kw = {"dtype": torch.float32, "device": x.device}
-            lp, ent, lse, stat = torch.empty(n, **kw), torch.empty(n, **kw), torch.empty(n, **kw), torch.empty(2, n, **kw)
-            top = torch.empty(n, top_k, **kw) if top_k else None
-            ids = torch.empty(n, top_k, dtype=torch.int64, device=x.device) if top_k else None
-            v = x.shape[1]
-            splits = native("pda_logprob_splits")(_i64(n), v, top_k) if v > 1024 else 1
-            part = keys = None
-            if splits > 1:      # long rows in parts, joined by a second launch
-                part = torch.empty(n, splits, 4, **kw)
-                keys = torch.empty(n, splits, top_k, dtype=torch.int64, device=x.device)
-            m = stat.data_ptr()
-            run_on(x, entry, "token_logprobs",
-                   _Args(x.data_ptr(), x.stride(0), n, v, tokens.data_ptr(), tokens.dtype == torch.int64, ignore, inv_t,
-                         inv_t * _LOG2E, top_k, lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), m, m + 4 * n, ptr(top),
-                         ptr(ids), None, None, None, None, splits, ptr(part), ptr(keys)))
+        lp, ent, lse, top, ids, stat = _forward(x, tokens, inv_t, top_k, ignore, True)
         ctx.save_for_backward(x, tokens, stat, ent)
         ctx.how = (inv_t, ignore)
         ctx.set_materialize_grads(False)
@@ -151,7 +156,11 @@ def token_logprobs(logits, tokens, temperature=1.0, top_k=0, ignore_index=-100):
     x = logits.reshape(-1, v) if logits.dim() != 2 else logits
     if x.stride(1) != 1 and v > 1:
         x = x.contiguous()
-    out = _TokenLogprobs.apply(x, tokens.reshape(-1).contiguous(), 1.0 / temperature, top_k, ignore_index)
+    tokens = tokens.reshape(-1).contiguous()
+    if x.requires_grad and torch.is_grad_enabled():
+        out = _TokenLogprobs.apply(x, tokens, 1.0 / temperature, top_k, ignore_index)
+    else:
+        out = _forward(x, tokens, 1.0 / temperature, top_k, ignore_index, False)[:5 if top_k else 3]
     if len(lead) != 1:
         out = [t.reshape(lead) for t in out[:3]] + [t.reshape(lead + (top_k,)) for t in out[3:]]
     return TokenLogprobs(*out) if top_k else TokenLogprobs(*out, None, None)

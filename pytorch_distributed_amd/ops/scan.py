@@ -6,10 +6,11 @@ The evaluator's return report (agent_params.evaluate_returns) runs on it.
 On CPU tensors the same functions compute the same formulas in torch, step by step.
 """
 import ctypes
+import functools
 
 import torch
 
-from ._seq import TYPE_CODES, check_floating, check_int, differentiable_once, native, ptr, run_on
+from ._seq import TYPE_CODES, check_floating, check_int, differentiable_once, launched, native, ptr, run_on
 
 GATES = ("decay", "logit")
 _vp, _i64, _int = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
@@ -85,11 +86,11 @@ def _backward_torch(x, gate, h0, n, logit, mix, reverse, dh, dlast):
     return dx, dg, carry
 
 
-def _plan(x):
-    """-> (carries, chunks): how the kernels cut x's steps (csrc/scan.hip scan_plan)"""
+@functools.lru_cache(maxsize=1024)
+def _plan(B, T, D, code):
+    """-> (carries, chunks): how the kernels cut the steps (csrc/scan.hip scan_plan), a function of the sizes"""
     out = (ctypes.c_int * 2)()
-    B, T, D = x.shape
-    native("pda_scan_plan")(B, T, D, TYPE_CODES[x.dtype], ctypes.byref(out, 0), ctypes.byref(out, 4))
+    launched(native("pda_scan_plan")(B, T, D, code, ctypes.byref(out, 0), ctypes.byref(out, 4)), "linear_scan")
     return out[0], out[1]
 
 
@@ -97,28 +98,45 @@ def _lengths(lengths, B, T):
     return torch.full((B,), T) if lengths is None else lengths.long().clamp(0, T)
 
 
+def _cube(t):
+    """[B, T] (or a state [B]) as one channel"""
+    return t.unsqueeze(-1) if t is not None else None
+
+
+def _sizes(x):
+    """-> (B, T, D), x's strides and whether it has a channel dimension"""
+    return (x.shape, x.stride(), True) if x.dim() == 3 else ((*x.shape, 1), (*x.stride(), 1), False)
+
+
+def _forward(x, gate, h0, lengths, how, keep):
+    """-> (h, last, carry); carry: the states that a backward pass starts from, if `keep`"""
+    (B, T, D), xs, wide = _sizes(x)
+    if x.device.type == "cpu":
+        if wide:
+            h, last, _ = _forward_torch(x, gate, h0, _lengths(lengths, B, T), *how)
+            return h, last, None
+        h, last, _ = _forward_torch(_cube(x), _cube(gate), _cube(h0), _lengths(lengths, B, T), *how)
+        return h.squeeze(2), last.squeeze(1), None
+    entry = native("pda_scan_fwd")
+    kw = {"dtype": torch.float32, "device": x.device}
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    last = torch.empty((B, D) if wide else B, **kw)
+    carries, chunks = _plan(B, T, D, TYPE_CODES[x.dtype])
+    carry = torch.empty(B, carries, D, **kw) if keep else None
+    sums = torch.empty(B, chunks, 2, D, **kw) if chunks > 1 else None
+    run_on(x, entry, "linear_scan",
+           _Args(x.data_ptr(), gate.data_ptr(), None, *xs, *(gate.stride() if wide else (*gate.stride(), 1)), 0, 0, 0, ptr(h0),
+                 None, ptr(lengths), lengths is not None and lengths.dtype == torch.int64, h.data_ptr(), last.data_ptr(),
+                 ptr(carry), ptr(sums), None, None, None, B, T, D, *how, chunks))
+    return h, last, carry
+
+
 class _LinearScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, h0, lengths, logit, mix, reverse):
-        B, T, D = x.shape
-        how = (logit, mix, reverse)
-        carry = None
-        if x.device.type == "cpu":
-            h, last, _ = _forward_torch(x, gate, h0, _lengths(lengths, B, T), *how)
-        else:
-            entry = native("pda_scan_fwd")
-            h = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
-            last = torch.empty(B, D, dtype=torch.float32, device=x.device)
-            carries, chunks = _plan(x)
-            if any(ctx.needs_input_grad):
-                carry = torch.empty(B, carries, D, dtype=torch.float32, device=x.device)
-            sums = torch.empty(B, chunks, 2, D, dtype=torch.float32, device=x.device) if chunks > 1 else None
-            run_on(x, entry, "linear_scan",
-                   _Args(x.data_ptr(), gate.data_ptr(), None, *x.stride(), *gate.stride(), 0, 0, 0, ptr(h0), None,
-                         ptr(lengths), lengths is not None and lengths.dtype == torch.int64, h.data_ptr(), last.data_ptr(),
-                         ptr(carry), ptr(sums), None, None, None, B, T, D, *how, chunks))
+        ctx.how = (logit, mix, reverse)
+        h, last, carry = _forward(x, gate, h0, lengths, ctx.how, True)
         ctx.save_for_backward(x, gate, h0, lengths, carry)
-        ctx.how = how
         ctx.set_materialize_grads(False)
         return h, last
 
@@ -126,24 +144,29 @@ class _LinearScan(torch.autograd.Function):
     @differentiable_once
     def backward(ctx, dh, dlast):
         x, gate, h0, lengths, carry = ctx.saved_tensors
-        none = (None,) * 7
         if dh is None and dlast is None:
-            return none
-        B, T, D = x.shape
+            return (None,) * 7
+        (B, T, D), xs, wide = _sizes(x)
         if x.device.type == "cpu":
-            dx, dg, dh0 = _backward_torch(x, gate, h0, _lengths(lengths, B, T), *ctx.how, dh, dlast)
+            n = _lengths(lengths, B, T)
+            if wide:
+                dx, dg, dh0 = _backward_torch(x, gate, h0, n, *ctx.how, dh, dlast)
+            else:
+                dx, dg, dh0 = (t.squeeze(-1) for t in _backward_torch(_cube(x), _cube(gate), _cube(h0), n, *ctx.how,
+                                                                      _cube(dh), _cube(dlast)))
         else:
             entry = native("pda_scan_bwd")
             dlast = dlast.contiguous() if dlast is not None else None
-            dx = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
-            dg, dh0 = torch.empty_like(dx), torch.empty(B, D, dtype=torch.float32, device=x.device)
-            chunks = _plan(x)[1]
-            sums = torch.empty(B, chunks, 2, D, dtype=torch.float32, device=x.device) if chunks > 1 else None
+            kw = {"dtype": torch.float32, "device": x.device}
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            dg, dh0 = torch.empty_like(dx), torch.empty((B, D) if wide else B, **kw)
+            chunks = _plan(B, T, D, TYPE_CODES[x.dtype])[1]
+            sums = torch.empty(B, chunks, 2, D, **kw) if chunks > 1 else None
+            ds = (0, 0, 0) if dh is None else dh.stride() if wide else (*dh.stride(), 1)
             run_on(x, entry, "linear_scan backward",
-                   _Args(x.data_ptr(), gate.data_ptr(), ptr(dh), *x.stride(), *gate.stride(),
-                         *(dh.stride() if dh is not None else (0, 0, 0)), ptr(h0), ptr(dlast), ptr(lengths),
-                         lengths is not None and lengths.dtype == torch.int64, None, None, ptr(carry), ptr(sums),
-                         dx.data_ptr(), dg.data_ptr(), dh0.data_ptr(), B, T, D, *ctx.how, chunks))
+                   _Args(x.data_ptr(), gate.data_ptr(), ptr(dh), *xs, *(gate.stride() if wide else (*gate.stride(), 1)), *ds,
+                         ptr(h0), ptr(dlast), ptr(lengths), lengths is not None and lengths.dtype == torch.int64, None, None,
+                         ptr(carry), ptr(sums), dx.data_ptr(), dg.data_ptr(), dh0.data_ptr(), B, T, D, *ctx.how, chunks))
         return dx, dg, (dh0 if h0 is not None else None), None, None, None, None
 
 
@@ -190,20 +213,21 @@ def linear_scan(x, gate, h0=None, gates="decay", mix=False, reverse=False, lengt
     if lengths is not None:
         check_int(lengths, "lengths", x.shape[:1], x.device)
         lengths = lengths.contiguous()
-    flat = x.dim() == 2
-    if flat:
-        x, gate, h0 = x.unsqueeze(2), gate.unsqueeze(2), h0.unsqueeze(1) if h0 is not None else None
-    if x.shape[0] * x.shape[2] >= 1 << 31 or x.shape[1] >= 1 << 31:
+    if x.shape[0] * (x.shape[2] if x.dim() == 3 else 1) >= 1 << 31 or x.shape[1] >= 1 << 30:
         raise ValueError("x of shape %s is too large" % (tuple(x.shape),))
     h0 = h0.contiguous() if h0 is not None else None
-    h, last = _LinearScan.apply(x, gate, h0, lengths, logit, int(bool(mix)), int(bool(reverse)))
-    return (h.squeeze(2), last.squeeze(1)) if flat else (h, last)
+    how = (logit, int(bool(mix)), int(bool(reverse)))
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
+        return _LinearScan.apply(x, gate, h0, lengths, *how)
+    return _forward(x, gate, h0, lengths, how, False)[:2]
 
 
 def _span(t):
     """The addresses [first, behind the last) of a 2-d tensor."""
-    (n0, n1), (s0, s1) = t.shape, t.stride()
     first = t.data_ptr()
+    if t.is_contiguous():
+        return first, first + t.element_size() * t.numel()
+    (n0, n1), (s0, s1) = t.shape, t.stride()
     return first, first + t.element_size() * ((n0 - 1) * s0 + (n1 - 1) * s1 + 1 if n0 and n1 else 0)
 
 
