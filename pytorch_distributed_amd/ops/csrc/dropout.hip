@@ -40,7 +40,9 @@ __device__ __forceinline__ uint32_t drop_group(const DropKey& k, long long g) {
     return keep;
 }
 
-// A thread takes 16 bytes (one or two groups of four) of each tensor at a time, DROP_U of them in flight.
+// A thread takes 16 bytes (one or two groups of four) of each tensor at a time, DROP_U of them in flight.  Bound by memory:
+// 16384 x 4096 bf16 with residual 70 us for 403 MB (5.7 TB/s), its backward pass 45 us for 268 MB (6.0 TB/s); a copy of 256
+// MB reaches 5.4.  128 x 512 fp32: 3.0 us, the launch.
 #define DROP_U 2
 template <typename T, bool RESIDUAL, bool STREAM>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs p) {

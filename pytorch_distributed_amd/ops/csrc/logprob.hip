@@ -212,6 +212,8 @@ __device__ __forceinline__ void lp_rank(const uint64_t* keys, int n, int top_k, 
 }
 
 // ---- rows of up to LP_SHORT tokens: G lanes hold E tokens each --------------------------------------------------------
+// One load, butterfly sums within the G lanes, no LDS.  Bound by the launch: 4096 x 18 fp32 (0.3 MB) 3.6 us forward, 3.2 us
+// backward, where the smallest launches of this file take 2.3.
 template <typename T, int E, int G>
 __global__ __launch_bounds__(256) void logprob_short_kernel(LogprobArgs p) {
     const int lane = threadIdx.x & 63, l = lane & (G - 1);
@@ -352,7 +354,7 @@ struct LpList {
 // more than it saves: 4096 rows 248 -> 277 us).
 //
 // 4096 x 32000 bf16 without alternatives: 48.4 us, 5.4 TB/s of the 5.4 to 5.7 that a copy or a sum of 256 MB reaches here.
-// 4096 x 131072 bf16 with 8 alternatives: 248 us, 4.3 TB/s (a sum of 1 GB: 4.0 to 4.4).  Split rows are bound by the
+// 4096 x 131072 bf16 with 8 alternatives: 248 us, 4.3 TB/s (a sum of 1 GB reads 4.0).  Split rows are bound by the
 // latency of the chain of loads, joins and the second launch: 1 x 131072 10.0 + 4.6 us.  (Workgroups of 1024 threads with a
 // shared limit, so that fewer parts are joined: 16 to 32 us.)
 template <typename T, bool TOP, bool FILL>
@@ -522,7 +524,9 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs p) {
 }
 
 // ---- gradient ----------------------------------------------------------------------------------------------------------
-// One pass: each logit read once, each gradient written once.
+// One pass: each logit read once, each gradient written once, nothing summed (p comes from the forward pass's statistics).
+// Bound by memory: 4096 x 32000 bf16 78 us for 524 MB, 6.7 TB/s, part of the logits still in the memory-side cache from the
+// forward pass (a copy of 262 MB reaches 5.4).
 struct LpGrad {
     LpRow q; float dent, dlp, k0, inv_t; long long tok; bool zero;
     __device__ __forceinline__ LpGrad(const LogprobArgs& p, long long row, bool short_row)
@@ -563,7 +567,7 @@ __global__ __launch_bounds__(256) void logprob_short_bwd_kernel(LogprobArgs p) {
         }
     }
 }
-#define LP_BWD_U 4      // 16-byte loads in flight per thread: 2 / 4 / 8 took 111 / 107 / 115 us at 4096 x 32000 bf16
+#define LP_BWD_U 4      // 16-byte loads in flight per thread (with cached stores 2 / 4 / 8 took 111 / 107 / 115 us)
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void logprob_long_bwd_kernel(LogprobArgs p, int parts) {
     constexpr int VEC = 16 / sizeof(T), U = LP_BWD_U;
