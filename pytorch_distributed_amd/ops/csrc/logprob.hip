@@ -353,7 +353,7 @@ struct LpList {
 // at once instead (1 row of 131072 bf16, 20 alternatives: 11.4 -> 10.0 us; in the loop over a whole row the same code costs
 // more than it saves: 4096 rows 248 -> 277 us).
 //
-// 4096 x 32000 bf16 without alternatives: 48.4 us, 5.4 TB/s of the 5.4 to 5.7 that a copy or a sum of 256 MB reaches here.
+// 4096 x 32000 bf16 without alternatives, a tenth of the rows ignored: 48.5 us for 236 MB, 4.9 TB/s (a sum of 256 MB: 5.7).
 // 4096 x 131072 bf16 with 8 alternatives: 248 us, 4.3 TB/s (a sum of 1 GB reads 4.0).  Split rows are bound by the
 // latency of the chain of loads, joins and the second launch: 1 x 131072 10.0 + 4.6 us.  (Workgroups of 1024 threads with a
 // shared limit, so that fewer parts are joined: 16 to 32 us.)
@@ -525,8 +525,8 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs p) {
 
 // ---- gradient ----------------------------------------------------------------------------------------------------------
 // One pass: each logit read once, each gradient written once, nothing summed (p comes from the forward pass's statistics).
-// Bound by memory: 4096 x 32000 bf16 78 us for 524 MB, 6.7 TB/s, part of the logits still in the memory-side cache from the
-// forward pass (a copy of 262 MB reaches 5.4).
+// Bound by memory: 4096 x 32000 bf16, a tenth of the rows ignored, 78 us for 498 MB, 6.4 TB/s, part of the logits still in
+// the memory-side cache from the forward pass (a copy of 256 MB reaches 5.4).
 struct LpGrad {
     LpRow q; float dent, dlp, k0, inv_t; long long tok; bool zero;
     __device__ __forceinline__ LpGrad(const LogprobArgs& p, long long row, bool short_row)

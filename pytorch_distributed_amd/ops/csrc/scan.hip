@@ -8,6 +8,7 @@
 // next to 1 would be repeated over the whole memory of the recurrence, while 1 - a keeps its own precision (and a does
 // below 1/2).  States are 32 bits wide throughout; h is rounded once, where it is stored in x's type.
 #include "seq.h"
+#include <type_traits>
 #pragma clang fp reassociate(off)       // h - c h must not become (1 - c) h
 
 struct ScanArgs {
@@ -63,14 +64,21 @@ __device__ __forceinline__ int scan_length(const ScanArgs& p, int b) {
 // gates and end state, and each chunk's workgroup folds those in front of it before it starts.  x and gate are then read
 // twice.
 //
-// Measured at 8 x 2048 x 2048 bf16, sigmoid gates, leaky average (256 workgroups, one per CU): forward 52.5 us for 201 MB
-// (3.8 TB/s), backward 102 us for 336 MB (3.3 TB/s); what is left is that loads, joins and stores of a tile follow one
-// another on a CU that holds one workgroup.  At 1 x 65521 x 512 fp32 (16 slabs, 256 chunks): 60 + 75 us forward for 268 +
-// 403 MB, 47 + 140 us backward for 268 + 671 MB, 4.5 to 5.7 TB/s: bound by memory, a third of it the second reading.
+// Measured at 8 x 2048 x 2048 bf16, sigmoid gates, leaky average, lengths of 1024 to 2048 (256 workgroups, one per CU):
+// forward 53 us for 168 MB (3.2 TB/s), backward 102 us for 285 MB (2.8 TB/s).  Loads, joins and stores of a tile follow one
+// another on a CU that holds one workgroup, and the longest sequence sets the time.  At 1 x 65521 x 512 fp32 (16 slabs, 256 workgroups): 54 + 78 us forward for 268 +
+// 403 MB, 47 + 140 us backward for 268 + 671 MB, 4.8 to 5.7 TB/s: bound by memory, a third of it the second reading.
 #define SCAN_CL 8
+// scan_sum_kernel, either direction: 128 / 256 / 512 threads take 65 + 62 / 54 + 47 / 60 + 50 us (forward + backward) at
+// 1 x 65521 x 512 fp32
+template <typename T> struct ScanSum {
+    typedef float Acc;
+    static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = 1, NT = 256;
+};
 // a forward tile holds a whole number of backward tiles: the forward pass leaves the state in front of each of those
 template <typename T> struct ScanFwd {
     typedef float Acc;
+    typedef ScanSum<T> Sum;
     static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = 32 / VEC, NT = 512;
 };
 template <typename T> struct ScanBwd {
@@ -81,8 +89,8 @@ template <typename T> struct ScanBwd {
 // there, so states and products are 64 bits wide: a constant gate such as 0.99 rounds every product the same way, which
 // left 5e-7 of 12500 discounted returns in 32 bits.
 // (16 x 12500 fp32 returns: 8.7 us, of which the loads of the two tiles that a workgroup walks are most.)
-struct ScanRow { typedef double Acc; static constexpr int VEC = 1, CL = 1, L = 8, NT = 1024; };
-struct ScanWave { typedef double Acc; static constexpr int VEC = 1, CL = 1, L = 8, NT = 64; };
+struct ScanRow { typedef double Acc; typedef ScanRow Sum; static constexpr int VEC = 1, CL = 1, L = 8, NT = 1024; };
+struct ScanWave { typedef double Acc; typedef void Sum; static constexpr int VEC = 1, CL = 1, L = 8, NT = 64; };
 // The lanes of a wave: SW consecutive ones hold consecutive runs of steps of one group of VEC channels, so that a scan
 // over steps moves along a DPP row.
 template <typename S> struct ScanLane {
@@ -648,13 +656,14 @@ template <typename T, typename F, typename B, bool LOGIT, bool MIX, int MODE>
 static void scan_launch(const ScanArgs& p, const ScanPlan& k, bool backward, hipStream_t stream) {
     constexpr int READ = MODE == SCAN_STREAM ? SCAN_WIDE : MODE;
     const dim3 grid((unsigned)((long long)p.B * k.slabs * k.chunks)), fwd(F::NT), bwd(B::NT);
-    if (!backward) {
-        if (k.chunks > 1) hipLaunchKernelGGL((scan_sum_kernel<T, F, LOGIT, MIX, true, READ>), grid, fwd, 0, stream, p);
-        hipLaunchKernelGGL((scan_fwd_kernel<T, F, LOGIT, MIX, MODE>), grid, fwd, 0, stream, p);
-    } else {
-        if (k.chunks > 1) hipLaunchKernelGGL((scan_sum_kernel<T, B, LOGIT, false, false, READ>), grid, bwd, 0, stream, p);
-        hipLaunchKernelGGL((scan_bwd_kernel<T, B, LOGIT, MIX, MODE>), grid, bwd, 0, stream, p);
+    typedef typename F::Sum Sum;
+    if constexpr (!std::is_same<F, ScanWave>::value) {      // (which never has chunks)
+        const dim3 sum(Sum::NT);
+        if (k.chunks > 1 && !backward) hipLaunchKernelGGL((scan_sum_kernel<T, Sum, LOGIT, MIX, true, READ>), grid, sum, 0, stream, p);
+        if (k.chunks > 1 && backward) hipLaunchKernelGGL((scan_sum_kernel<T, Sum, LOGIT, false, false, READ>), grid, sum, 0, stream, p);
     }
+    if (!backward) hipLaunchKernelGGL((scan_fwd_kernel<T, F, LOGIT, MIX, MODE>), grid, fwd, 0, stream, p);
+    else hipLaunchKernelGGL((scan_bwd_kernel<T, B, LOGIT, MIX, MODE>), grid, bwd, 0, stream, p);
 }
 template <typename T, typename F, typename B, int MODE>
 static void scan_forms(const ScanArgs& p, const ScanPlan& k, bool backward, hipStream_t stream) {

@@ -117,6 +117,31 @@ def test_a_replayed_counter_draws_new_masks():
         assert torch.equal(y, want) and torch.equal(d, want)
 
 
+@pytest.mark.parametrize("kind", ["logprob", "scan_long", "returns", "dropout"])
+def test_calls_without_gradients_replay_what_calls_with_them_give(kind):
+    from pytorch_distributed_amd.ops.dropout import dropout
+    from pytorch_distributed_amd.ops.logprob import token_logprobs
+    from pytorch_distributed_amd.ops.scan import linear_scan
+    ctr, tok = torch.full((1,), 7, dtype=torch.int64, device="cuda"), torch.arange(5, device="cuda")
+    gate = rand((3, 9000), torch.float32, 5, 1.5, 2.0)
+    x, f = {"logprob": (rand((5, 9000), torch.bfloat16, 0), lambda t: token_logprobs(t, tok, top_k=6)),
+            "scan_long": (rand((1, 6000, 40), torch.bfloat16, 1),
+                          lambda t: linear_scan(t, torch.full_like(t, 0.75), mix=True)),
+            "returns": (rand((3, 9000), torch.float32, 2), lambda t: linear_scan(t, gate, gates="logit", reverse=True)),
+            "dropout": (rand((33, 515), torch.bfloat16, 3), lambda t: (dropout(t, 0.3, 5, ctr, residual=t),))}[kind]
+    with torch.no_grad():
+        graph, out = capture(lambda: f(x))
+    for seed in range(4):
+        x.copy_(rand(x.shape, x.dtype, 20 + seed))
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        want = f(x.clone().requires_grad_())
+        assert any(t.requires_grad for t in want)
+        same(got, [t.detach() for t in want])
+        torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("kind", ["logprob", "scan", "scan_long", "returns"])
 def test_two_graphs_at_once(kind):
     """Two captured calls share no scratch: replayed side by side on two streams they keep their results."""

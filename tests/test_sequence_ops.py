@@ -707,6 +707,24 @@ def policy_data(dev, b=3, t=21, d=24, v=37):
 
 
 @on_devices
+def test_calls_without_gradients(dev):
+    """Calls that need no gradient take a shorter way to the same kernels: same results, and outputs free to be written."""
+    x, g = rand((3, 700, 12), torch.float32, dev, 0), torch.sigmoid(rand((3, 700, 12), torch.float32, dev, 1))
+    tok, ctr, n = torch.arange(3, device=dev)[:, None].expand(3, 700), counter_at(4, dev), torch.tensor([700, 0, 33], device=dev)
+    for f in (lambda t: token_logprobs(t, tok, temperature=0.5, top_k=4), lambda t: token_logprobs(t, tok)[:3],
+              lambda t: linear_scan(t, g, lengths=n), lambda t: linear_scan(t[:, :, 0], g[:, :, 0], reverse=True, lengths=n),
+              lambda t: (dropout(t, 0.25, 1, ctr),), lambda t: (dropout(t, 0.25, 1, ctr, residual=t),)):
+        want = f(x.clone().requires_grad_())
+        with torch.no_grad():
+            inside = f(x.clone().requires_grad_())
+        outside = f(x)
+        for w, a, b in zip(want, inside, outside):
+            assert torch.equal(w, a) and torch.equal(w, b) and not a.requires_grad and not b.requires_grad
+            assert w.shape == b.shape and w.stride() == b.stride()
+            b.zero_()
+
+
+@on_devices
 @pytest.mark.parametrize("op", ("logprob", "scan", "dropout"))
 def test_gradients_are_not_differentiated_again(dev, op):
     """A graph of the gradient may be asked for (as a larger graph does); going through it is refused, not wrong."""
