@@ -2,6 +2,7 @@
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import lib, native_error
 
@@ -40,6 +41,16 @@ def differentiable_once(backward):
     def run(ctx, *grads):
         return (with_graph if torch.is_grad_enabled() else backward)(ctx, *grads)
     return run
+
+
+def wants_graph(*tensors):
+    """Whether a call has to go through autograd: a gradient may be asked of it, or tangents are being carried forward (which
+    the operators' functions refuse)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return getattr(forward_ad, "_current_level", -1) >= 0
 
 
 def ptr(t):

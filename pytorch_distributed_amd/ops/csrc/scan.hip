@@ -702,7 +702,8 @@ static int scan_run(const ScanArgs* args, int dtype, bool backward, hipStream_t 
     p.chunk_len = k.chunk_len;
     p.carry_len = k.carry_len;
     p.carries = k.carries;
-    if ((long long)p.B * k.slabs * k.chunks >= (1ll << 32) / ScanFwd<elem_f32>::NT) return SEQ_REFUSED;    // (a launch's threads)
+    const int nt = k.kind == SCAN_KIND_WAVE ? ScanWave::NT : k.kind == SCAN_KIND_ROW ? ScanRow::NT : ScanFwd<elem_f32>::NT;
+    if ((long long)p.B * k.slabs * k.chunks >= (1ll << 32) / nt) return SEQ_REFUSED;    // (a launch's threads)
     if (dtype == SEQ_F32) scan_dispatch<elem_f32>(p, k, backward, stream);
     else if (dtype == SEQ_BF16) scan_dispatch<elem_bf16>(p, k, backward, stream);
     else scan_dispatch<elem_f16>(p, k, backward, stream);

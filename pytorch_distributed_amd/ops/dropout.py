@@ -11,7 +11,7 @@ import ctypes
 import torch
 import torch.nn as nn
 
-from ._seq import check_floating, differentiable_once, native, ptr, run_on
+from ._seq import check_floating, differentiable_once, native, ptr, run_on, wants_graph
 
 _M64 = (1 << 64) - 1
 _GOLDEN = 0x9E3779B97F4A7C15
@@ -116,7 +116,7 @@ def dropout(x, p, seed, counter, site=0, residual=None):
                 residual.device != x.device:
             raise ValueError("residual must have x's shape, type and device")
     counter = counter if counter.dim() == 1 else counter.reshape(1)
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if wants_graph(x, residual):
         return _Dropout.apply(x, residual, p, seed, site, counter)
     return _run(x.contiguous(), residual.contiguous() if residual is not None else None, p, seed, site, counter, None)
 

@@ -11,7 +11,7 @@ from collections import namedtuple
 
 import torch
 
-from ._seq import check_floating, check_int, differentiable_once, native, ptr, run_on
+from ._seq import check_floating, check_int, differentiable_once, native, ptr, run_on, wants_graph
 
 MAX_TOP = 32        # csrc/logprob.hip LP_MAX_TOP
 TokenLogprobs = namedtuple("TokenLogprobs", "logprob, entropy, logsumexp, top_logprobs, top_tokens")
@@ -157,7 +157,7 @@ def token_logprobs(logits, tokens, temperature=1.0, top_k=0, ignore_index=-100):
     if x.stride(1) != 1 and v > 1:
         x = x.contiguous()
     tokens = tokens.reshape(-1).contiguous()
-    if x.requires_grad and torch.is_grad_enabled():
+    if wants_graph(x):
         out = _TokenLogprobs.apply(x, tokens, 1.0 / temperature, top_k, ignore_index)
     else:
         out = _forward(x, tokens, 1.0 / temperature, top_k, ignore_index, False)[:5 if top_k else 3]

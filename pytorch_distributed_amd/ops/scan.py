@@ -10,7 +10,7 @@ import functools
 
 import torch
 
-from ._seq import TYPE_CODES, check_floating, check_int, differentiable_once, launched, native, ptr, run_on
+from ._seq import TYPE_CODES, check_floating, check_int, differentiable_once, launched, native, ptr, run_on, wants_graph
 
 GATES = ("decay", "logit")
 _vp, _i64, _int = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
@@ -186,7 +186,8 @@ def linear_scan(x, gate, h0=None, gates="decay", mix=False, reverse=False, lengt
     """-> (h, last): h_t = a_t h_{t-1} + u_t along dimension 1.
 
     x, gate    [B, T, D] (or [B, T]: one channel), float32, bfloat16 or float16, of one type; any strides, so a gate
-               shared by steps or channels may be passed as an expanded view (its gradient is summed by autograd)
+               shared by steps or channels may be passed as an expanded view (its gradient is summed by autograd);
+               on a GPU up to 8 million sequences times groups of 32 channels
     gates      "decay": a = gate  |  "logit": a = sigmoid(gate)
     mix        False: u = x  |  True: u = (1 - a) x (a leaky average)
     h0         [B, D] (or [B]) float32 state in front of the first step, None = 0
@@ -217,7 +218,7 @@ def linear_scan(x, gate, h0=None, gates="decay", mix=False, reverse=False, lengt
         raise ValueError("x of shape %s is too large" % (tuple(x.shape),))
     h0 = h0.contiguous() if h0 is not None else None
     how = (logit, int(bool(mix)), int(bool(reverse)))
-    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
+    if wants_graph(x, gate, h0):
         return _LinearScan.apply(x, gate, h0, lengths, *how)
     return _forward(x, gate, h0, lengths, how, False)[:2]
 

@@ -707,6 +707,18 @@ def policy_data(dev, b=3, t=21, d=24, v=37):
 
 
 @on_devices
+def test_tangents_are_refused(dev):
+    """Forward-mode differentiation is not offered: an error, not a result without its tangent."""
+    from torch.autograd import forward_ad
+    x, tok = rand((3, 8), torch.float32, dev, 0), torch.zeros(3, dtype=torch.int64, device=dev)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for f in (lambda: token_logprobs(d, tok), lambda: linear_scan(d, x), lambda: dropout(d, 0.5, 1, counter_at(0, dev))):
+            with pytest.raises(RuntimeError):       # (NotImplementedError is one)
+                f()
+
+
+@on_devices
 def test_calls_without_gradients(dev):
     """Calls that need no gradient take a shorter way to the same kernels: same results, and outputs free to be written."""
     x, g = rand((3, 700, 12), torch.float32, dev, 0), torch.sigmoid(rand((3, 700, 12), torch.float32, dev, 1))
