@@ -189,17 +189,21 @@ __device__ __forceinline__ void scan_fetch(Raw<T, S::VEC> (&r)[S::L], const T* b
         else r[l] = none;
     }
 }
+// on = false stores zeros (whole words of them: half the selects of 16-bit elements one by one)
 template <typename T, int VEC, int MODE>
-__device__ __forceinline__ void scan_store(T* row, const float (&v)[VEC], int nch) {
+__device__ __forceinline__ void scan_store(T* row, const float (&v)[VEC], int nch, bool on) {
     if constexpr (MODE != SCAN_ANY && VEC != 1) {
         vec16<T> o;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o.e[i] = from_f32<T>(v[i]);
-        store16<MODE == SCAN_STREAM>(row, o);
+        seq_u32x4 w = __builtin_bit_cast(seq_u32x4, o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = on ? w[i] : 0u;
+        store16<MODE == SCAN_STREAM>(row, __builtin_bit_cast(vec16<T>, w));
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
-            if (i < nch) row[i] = from_f32<T>(v[i]);
+            if (i < nch) row[i] = from_f32<T>(on ? v[i] : 0.f);
     }
 }
 // joins a later part (a, h) behind an earlier one (pa, ph): state -> a (pa state + ph) + h
@@ -221,6 +225,10 @@ template <int O, bool UP, int BANKS = 0xf, typename Acc>
 __device__ __forceinline__ Acc dpp_shift(Acc none, Acc v) {             // lane i of a row of 16 gets lane i -+ O's, or `none`
     return dpp_move<(UP ? 0x110 : 0x100) + O, BANKS>(none, v);
 }
+template <int O, bool UP>
+__device__ __forceinline__ float dpp_neighbour(float v) {               // the same without `none`: lanes that have no such neighbour are
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), (UP ? 0x110 : 0x100) + O, 0xf, 0xf, true));
+}                                                                       // replaced by the caller (saves a move each)
 template <bool UP, typename Acc>
 __device__ __forceinline__ Acc wave_shift(Acc v) {                      // lane i of the wave gets lane i -+ 1's
     return dpp_move<UP ? 0x138 : 0x130, 0xf>((Acc)0, v);
@@ -236,12 +244,17 @@ template <int O, int SW, bool UP, typename Acc>
 __device__ __forceinline__ void scan_lanes_step(Acc& A, Acc& H) {
     if constexpr (O < SW) {
         constexpr int BANKS = SW == 8 && O == 4 ? (UP ? 0xa : 0x5) : 0xf;      // (the lanes of a group that have a partner)
-        Acc pa = dpp_shift<O, UP, BANKS>((Acc)1, A), ph = dpp_shift<O, UP, BANKS>((Acc)0, H);
-        if (SW < 16 && BANKS == 0xf) {
+        Acc pa, ph;
+        if constexpr (SW < 16 && BANKS == 0xf) {
             const int i = threadIdx.x & (SW - 1);
             const bool on = UP ? i >= O : i < SW - O;
+            pa = dpp_neighbour<O, UP>(A);
+            ph = dpp_neighbour<O, UP>(H);
             pa = on ? pa : (Acc)1;
             ph = on ? ph : (Acc)0;
+        } else {
+            pa = dpp_shift<O, UP, BANKS>((Acc)1, A);
+            ph = dpp_shift<O, UP, BANKS>((Acc)0, H);
         }
         SCAN_JOIN(A, H, pa, ph);
     }
@@ -287,8 +300,8 @@ __device__ __forceinline__ void scan_across(Acc (&A)[S::VEC], Acc (&H)[S::VEC], 
     for (int v = 0; v < S::VEC; ++v) {      // exclusive: the neighbour's
         Acc pa, ph;
         if constexpr (SW <= 16) {
-            pa = dpp_shift<1, UP>((Acc)1, A[v]);
-            ph = dpp_shift<1, UP>((Acc)0, H[v]);
+            pa = dpp_neighbour<1, UP>(A[v]);
+            ph = dpp_neighbour<1, UP>(H[v]);
         } else {
             pa = wave_shift<UP>(A[v]);
             ph = wave_shift<UP>(H[v]);
@@ -417,8 +430,8 @@ __global__ __launch_bounds__(S::NT) void scan_fwd_kernel(ScanArgs p) {
             const long long t = on && p.reverse ? w.n - 1 - i : i;
             float o[VEC];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) o[v] = on ? (float)acc_fma(A[l][v], h[v], H[l][v]) : 0.f;
-            scan_store<T, VEC, MODE>(out + t * p.D, o, w.nch);
+            for (int v = 0; v < VEC; ++v) o[v] = (float)acc_fma(A[l][v], h[v], H[l][v]);
+            scan_store<T, VEC, MODE>(out + t * p.D, o, w.nch, on);
         }
     }
     if (w.chunk == p.chunks - 1 && sub == 0) {
@@ -516,11 +529,11 @@ __global__ __launch_bounds__(S::NT) void scan_bwd_kernel(ScanArgs p) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 const float G = (float)acc_fma(P[l][v], h[v], q[l][v]);
-                ox[v] = on ? (MIX ? G * cc[l][v] : G) : 0.f;
-                og[v] = on ? G * wt[l][v] : 0.f;
+                ox[v] = MIX ? G * cc[l][v] : G;
+                og[v] = G * wt[l][v];
             }
-            scan_store<T, VEC, MODE>((T*)p.dx + base + t * p.D, ox, w.nch);
-            scan_store<T, VEC, MODE>((T*)p.dg + base + t * p.D, og, w.nch);
+            scan_store<T, VEC, MODE>((T*)p.dx + base + t * p.D, ox, w.nch, on);
+            scan_store<T, VEC, MODE>((T*)p.dg + base + t * p.D, og, w.nch, on);
         }
     }
     if (w.chunk == 0 && sub == 0) {
