@@ -65,8 +65,9 @@ __device__ __forceinline__ int scan_length(const ScanArgs& p, int b) {
 // twice.
 //
 // Measured at 8 x 2048 x 2048 bf16, sigmoid gates, leaky average, lengths of 1024 to 2048 (256 workgroups, one per CU):
-// forward 53 us for 168 MB (3.2 TB/s), backward 102 us for 285 MB (2.8 TB/s).  Loads, joins and stores of a tile follow one
-// another on a CU that holds one workgroup, and the longest sequence sets the time.  At 1 x 65521 x 512 fp32 (16 slabs, 256 workgroups): 54 + 78 us forward for 268 +
+// forward 53 us for 168 MB (3.2 TB/s), backward 98 us for 285 MB (2.9 TB/s).  Loads, arithmetic and stores of a tile follow
+// one another on a CU that holds one workgroup (backward: one wave per SIMD, which issues about 2500 vector instructions a
+// tile, 10000 of the tile's 15000 cycles), and the longest sequence sets the time.  At 1 x 65521 x 512 fp32 (16 slabs, 256 workgroups): 54 + 78 us forward for 268 +
 // 403 MB, 47 + 140 us backward for 268 + 671 MB, 4.8 to 5.7 TB/s: bound by memory, a third of it the second reading.
 #define SCAN_CL 8
 // scan_sum_kernel, either direction: 128 / 256 / 512 threads take 65 + 62 / 54 + 47 / 60 + 50 us (forward + backward) at
