@@ -169,6 +169,21 @@ def test_logprob_alternatives_in_hard_orders(dev, dt, order, v, k):
 
 @on_devices
 @on_types
+@pytest.mark.parametrize("order", ["up", "down", "equal", "ties", "steps", "masked", "nearly empty"])
+@pytest.mark.parametrize("v,k", [(20003, 32), (8192, 5)])
+def test_logprob_alternatives_in_hard_orders_of_split_rows(dev, dt, order, v, k):
+    """Rows cut into parts: more equal values, or values above a part's limit, than a wave can order at once; parts with fewer
+    tokens left than alternatives are asked for."""
+    i = torch.arange(v)
+    row = {"up": torch.linspace(-4, 4, v), "down": torch.linspace(4, -4, v), "equal": torch.ones(v), "ties": (i * 7919 % 11).float(),
+           "steps": (i // 700).float(), "masked": torch.where(i % 300 == 7, i / v, torch.full((v,), -INF)),
+           "nearly empty": torch.where((i == 3) | (i == v - 1), torch.ones(v), torch.full((v,), -INF))}[order]
+    x = row.to(dt).expand(3, v).contiguous().to(dev)
+    check_logprob(x, torch.tensor([3, 7, v - 1], device=dev), k=k, grads=False)
+
+
+@on_devices
+@on_types
 def test_logprob_strides_and_shapes(dev, dt):
     big = rand((10, 1000), dt, dev, 3, 2.0)
     tokens = torch.arange(5, device=dev)
@@ -734,6 +749,42 @@ def test_calls_without_gradients(dev):
             assert torch.equal(w, a) and torch.equal(w, b) and not a.requires_grad and not b.requires_grad
             assert w.shape == b.shape and w.stride() == b.stride()
             b.zero_()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ("logprob", "scan", "dropout"))
+def test_offsets_past_32_bits(op):
+    """More than 2^31 elements: the last part of the tensor equals the same part taken alone."""
+    def noise(*shape):
+        return torch.empty(shape, dtype=torch.bfloat16, device="cuda").normal_()
+
+    if op == "logprob":
+        x, tok = noise(33000, 65540), torch.arange(33000, device="cuda")
+        part = slice(32000, 33000)      # (more than 512 rows: not split in either call)
+
+        def run(sl):
+            leaf = x[sl].detach().requires_grad_()
+            o = token_logprobs(leaf, tok[sl], top_k=3)
+            return o.logprob, o.top_tokens, torch.autograd.grad(o.logprob.sum() + o.entropy.sum(), leaf)[0]
+    elif op == "scan":
+        x, g = noise(3, 45000, 16384), torch.rand((1, 45000, 16384), dtype=torch.float32, device="cuda").to(torch.bfloat16)
+        part = slice(2, 3)
+
+        def run(sl):
+            leaf = x[sl].detach().requires_grad_()
+            h, last = linear_scan(leaf, g.expand(leaf.shape))
+            return h, last, torch.autograd.grad(h.sum(), leaf)[0]
+    else:
+        n = (1 << 31) + (1 << 22)
+        y = dropout(torch.ones(n, dtype=torch.bfloat16, device="cuda"), 0.5, 3, counter_at(1, "cuda"))
+        for at in (0, (1 << 31) - 2048, n - 4096):
+            want = 2 * oracle.keep_mask(range(at, at + 4096), 0.5, 3, 1, 0).astype(np.float64)
+            assert np.array_equal(np64(y[at:at + 4096]), want)
+        return
+    assert x.numel() > 1 << 31
+    whole = run(slice(None))
+    for a, b in zip(whole, run(part)):
+        assert torch.equal(a[part], b)
 
 
 @on_devices
