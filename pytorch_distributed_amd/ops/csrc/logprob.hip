@@ -68,6 +68,7 @@ __device__ __forceinline__ float lp_ref(float m, float c) {
     asm("" : "+v"(r));          // r is this rounded product wherever it is used: no contraction into an fma
     return r;
 }
+__device__ __forceinline__ bool lp_near(float r) { return fabsf(r) < LP_NEAR; }
 // `st` seen from the maximum m >= st.m (no part of it may turn into 0 * inf: the shift is cut off where 2^shift is 0)
 __device__ __forceinline__ LpStat lp_shift(LpStat st, float m, float c) {
     const float d = st.m == m ? 0.f : fmaxf(lp_ref(st.m, c) - lp_ref(m, c), -1.0e20f), e = lp_exp2(d);
@@ -115,7 +116,7 @@ struct LpRow {
     float m, r, c, l2; bool near, empty;
     __device__ __forceinline__ LpRow(float m_, float l2_, float c_, bool short_row) : m(m_), c(c_), l2(l2_) {
         r = lp_ref(m, c);
-        near = !short_row && fabsf(r) < LP_NEAR;
+        near = !short_row && lp_near(r);
         empty = m == -INFINITY && l2 == l2;     // nothing but -inf
     }
     __device__ __forceinline__ float log2p(float x) const { return (near ? __builtin_fmaf(x, c, -r) : (x - m) * c) - l2; }
@@ -164,10 +165,13 @@ __device__ __forceinline__ void lp_walk_row(const LogprobArgs& p, long long row,
     __syncthreads();
     m = fmaxf(fmaxf(part[0].m, part[1].m), fmaxf(part[2].m, part[3].m));
     bad = part[0].s + part[1].s + part[2].s + part[3].s;
+    // the form of d that LpRow, here and in the backward pass, takes for this maximum: s is relative to it
+    const float r = lp_ref(m, p.c);
+    const bool near = lp_near(r);
     float s = bad, u = 0.f;
     if (m > -INFINITY)
         for (int i = tid; i < p.vocab; i += 256) {
-            const float d = (to_f32(x[i]) - m) * p.c, e = lp_exp2(d);
+            const float v = to_f32(x[i]), d = near ? __builtin_fmaf(v, p.c, -r) : (v - m) * p.c, e = lp_exp2(d);
             s += e;
             u += e > 0.f ? e * d : 0.f;
         }
@@ -177,7 +181,7 @@ __device__ __forceinline__ void lp_walk_row(const LogprobArgs& p, long long row,
     if (lane == 0) part[wave] = LpStat{m, s, u};
     __syncthreads();
     const LpStat st{m, (part[0].s + part[1].s) + (part[2].s + part[3].s), (part[0].u + part[1].u) + (part[2].u + part[3].u)};
-    LpRow q(m, lp_log2_sum(st), p.c, true);
+    const LpRow q(m, lp_log2_sum(st), p.c, false);
     if (tid == 0) lp_finish_row(p, row, xt, st, q);
     uint64_t last = ~0ull;
     for (int k = 0; k < p.top_k; ++k) {
@@ -197,7 +201,7 @@ __device__ __forceinline__ void lp_walk_row(const LogprobArgs& p, long long row,
     __syncthreads();
 }
 __device__ __forceinline__ bool lp_ordinary(LpStat st, float c) {
-    return st.s > 0.f && st.s < INFINITY && fabsf(lp_ref(st.m, c)) < LP_NEAR;
+    return st.s > 0.f && st.s < INFINITY && lp_near(lp_ref(st.m, c));
 }
 // The top_k largest of n distinct keys (0: none) in LDS, by counting what is above each: whole workgroup
 template <typename F>

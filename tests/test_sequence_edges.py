@@ -1,0 +1,34 @@
+"""Rows, lengths and layouts of the sequence-policy operators that lie off the ordinary paths of their kernels (ops/logprob.py,
+ops/scan.py, ops/dropout.py), and calls that have to be refused."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from test_sequence_ops import check_logprob, on_devices, on_types, rand  # noqa: E402
+
+
+# ---- token log-probabilities ---------------------------------------------------------------------------------------
+def masked_rows(v, dt, dev, top, fill):
+    """Five rows of which a part is left, the rest `fill`; -> (logits, the tokens asked for)"""
+    x = torch.full((5, v), fill, dtype=dt)
+    live = rand((5, v), torch.float32, "cpu", v, 3.0, top).to(dt)
+    where = torch.zeros(5, v, dtype=torch.bool)
+    where[0, :200] = True
+    where[1, v // 2:v // 2 + 300] = True
+    where[2, ::2] = True
+    where[3, 7::500] = True
+    where[4, v // 3:] = True
+    return torch.where(where, live, x).to(dev), torch.tensor([5, v // 2 + 3, 8, 507, v - 1], device=dev)
+
+
+@on_devices
+@on_types
+@pytest.mark.parametrize("v", [2500, 20000])
+@pytest.mark.parametrize("top", [1e4, 6e4, 1e6])
+def test_logprob_rows_masked_with_the_lowest_value(dev, dt, v, top):
+    """Large logits among masks: forward and backward pass measure a row's exponents from the same rounded reference."""
+    x, tokens = masked_rows(v, dt, dev, min(top, 6e4) if dt == torch.float16 else top, torch.finfo(dt).min)
+    check_logprob(x, tokens, k=5)
