@@ -59,8 +59,9 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 // d = x c - r
 struct LpStat { float m, s, u; };
 #define LP_LN2 0.693147180559945309f
-// The rounding of r is at most |r| 2^-24: below this bound 2^(its rounding) stays near 1.  Rows beyond it (logits of more
-// than 7e6 T, masks of the type's lowest value in every place) are walked once more with d = (x - m) c.
+// The rounding of r is at most |r| 2^-24: below this bound 2^(its rounding) stays near 1.  Beyond it d = (x - m) c: in a part
+// that holds nothing but masks of a low value, and in rows whose maximum lies there (logits of more than 7e6 T, masks in
+// every place), which are walked once more because their parts' references cannot be told apart.
 #define LP_NEAR 1.0e7f
 __device__ __forceinline__ float lp_exp2(float d) { return __builtin_amdgcn_exp2f(d); }
 __device__ __forceinline__ float lp_ref(float m, float c) {
@@ -69,7 +70,8 @@ __device__ __forceinline__ float lp_ref(float m, float c) {
     return r;
 }
 __device__ __forceinline__ bool lp_near(float r) { return fabsf(r) < LP_NEAR; }
-// `st` seen from the maximum m >= st.m (no part of it may turn into 0 * inf: the shift is cut off where 2^shift is 0)
+// `st` seen from the maximum m >= st.m (no part of it turns into 0 * inf: the shift is cut off where 2^shift is 0, and s, a
+// count of at most the row's tokens up to r's rounding, is finite)
 __device__ __forceinline__ LpStat lp_shift(LpStat st, float m, float c) {
     const float d = st.m == m ? 0.f : fmaxf(lp_ref(st.m, c) - lp_ref(m, c), -1.0e20f), e = lp_exp2(d);
     return LpStat{m, st.s * e, e * __builtin_fmaf(d, st.s, st.u)};
@@ -86,11 +88,20 @@ __device__ __forceinline__ void lp_add(LpStat& st, const float (&x)[NX], float b
     st = lp_shift(st, fmaxf(st.m, bm), c);
     const float r = st.m == -INFINITY ? 0.f : lp_ref(st.m, c);
     float s = 0.f, u = 0.f;
+    if (lp_near(r)) {
 #pragma unroll
-    for (int i = 0; i < NX; ++i) {
-        const float d = __builtin_fmaf(x[i], c, -r), e = lp_exp2(d);
-        s += e;                                             // (NaN for a NaN)
-        u = __builtin_fmaf(e, fmaxf(d, -1000.f), u);        // (0 for -inf)
+        for (int i = 0; i < NX; ++i) {
+            const float d = __builtin_fmaf(x[i], c, -r), e = lp_exp2(d);
+            s += e;                                             // (NaN for a NaN)
+            u = __builtin_fmaf(e, fmaxf(d, -1000.f), u);        // (0 for -inf)
+        }
+    } else {        // nothing but masks of a low value so far (or a row that will be walked): s stays finite, and a larger maximum drops it
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+            const float d = (x[i] - st.m) * c, e = lp_exp2(d);
+            s += e;
+            u = __builtin_fmaf(e, fmaxf(d, -1000.f), u);
+        }
     }
     st.s += s;
     st.u += u;

@@ -7,7 +7,9 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_sequence_ops import check_logprob, on_devices, on_types, rand  # noqa: E402
+from test_sequence_ops import INF, check_logprob, on_devices, on_types, rand  # noqa: E402
+
+from pytorch_distributed_amd.ops.logprob import token_logprobs  # noqa: E402
 
 
 # ---- token log-probabilities ---------------------------------------------------------------------------------------
@@ -32,3 +34,21 @@ def test_logprob_rows_masked_with_the_lowest_value(dev, dt, v, top):
     """Large logits among masks: forward and backward pass measure a row's exponents from the same rounded reference."""
     x, tokens = masked_rows(v, dt, dev, min(top, 6e4) if dt == torch.float16 else top, torch.finfo(dt).min)
     check_logprob(x, tokens, k=5)
+
+
+@on_devices
+@on_types
+@pytest.mark.parametrize("v", [700, 2500, 20000])
+def test_logprob_masks_by_a_low_value_are_masks(dev, dt, v):
+    """A mask of a low finite value is a mask of -inf, bit for bit: such rows take the one pass that others take, whose sums run
+    in another order than those of a row that is walked again."""
+    def run(fill):
+        x, tokens = masked_rows(v, dt, dev, 1.0, fill)
+        x.requires_grad_()
+        o = token_logprobs(x, tokens, top_k=2)          # (every row has two tokens left)
+        d, = torch.autograd.grad(o.logprob.sum() + o.entropy.sum() + o.logsumexp.sum(), x)
+        return [o.logprob, o.entropy, o.logsumexp, o.top_logprobs, o.top_tokens, d]
+    want = run(-INF)
+    for fill in (torch.finfo(dt).min, -3e4) + (() if dt == torch.float16 else (-1e9, -1e20)):
+        for a, b in zip(run(fill), want):
+            assert torch.equal(a, b), fill
