@@ -9,6 +9,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.graph import increment_version
 
 from ._seq import TYPE_CODES, check_floating, check_int, differentiable_once, launched, native, ptr, run_on, wants_graph
 
@@ -271,4 +272,5 @@ def linear_scan_step(x, gate, state, gates="decay", mix=False, state_out=None):
     run_on(x, entry, "linear_scan_step",
            _StepArgs(x.data_ptr(), gate.data_ptr(), state.data_ptr(), out.data_ptr(), h.data_ptr(), *x.stride(),
                      *gate.stride(), *state.stride(), *out.stride(), B, D, logit, bool(mix)))
+    increment_version(out)      # (written behind torch's back: a graph that saved it has to notice)
     return h

@@ -10,6 +10,7 @@ sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from test_sequence_ops import INF, check_logprob, on_devices, on_types, rand  # noqa: E402
 
 from pytorch_distributed_amd.ops.logprob import token_logprobs  # noqa: E402
+from pytorch_distributed_amd.ops.scan import linear_scan_step  # noqa: E402
 
 
 # ---- token log-probabilities ---------------------------------------------------------------------------------------
@@ -52,3 +53,22 @@ def test_logprob_masks_by_a_low_value_are_masks(dev, dt, v):
     for fill in (torch.finfo(dt).min, -3e4) + (() if dt == torch.float16 else (-1e9, -1e20)):
         for a, b in zip(run(fill), want):
             assert torch.equal(a, b), fill
+
+
+# ---- linear recurrence ---------------------------------------------------------------------------------------------
+@on_devices
+@pytest.mark.parametrize("second_buffer", [False, True])
+def test_a_state_that_a_graph_saved_is_not_overwritten_unseen(dev, second_buffer):
+    x, g, state = rand((3, 8), torch.float32, dev, 1), torch.full((3, 8), 0.5, device=dev), rand((3, 8), torch.float32, dev, 2)
+    w = torch.ones(3, 8, device=dev, requires_grad=True)
+    out = torch.zeros(3, 8, device=dev) if second_buffer else state
+    y = (out * w).sum()                 # saves the buffer that the step writes
+    before = out._version
+    linear_scan_step(x, g, state, state_out=out if second_buffer else None)
+    assert out._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():        # tensors without a version counter
+        a = state.clone()
+        b = linear_scan_step(x, g, a)
+        assert torch.equal(a, b)
