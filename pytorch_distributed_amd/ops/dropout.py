@@ -63,7 +63,7 @@ def _run(x, residual, p, seed, site, counter, used):
         keep = keep_mask(x.numel(), p, seed, counter, site).reshape(x.shape)
         y = torch.where(keep, x.float() * scale, torch.zeros(()))
         return (y if residual is None else y + residual.float()).to(x.dtype)
-    entry = native("pda_dropout")
+    entry = native("pda_dropout", whole=used is not None)
     hi, lo = _threshold(p)
     y = torch.empty_like(x)
     args = _Args(ptr(x), ptr(residual), ptr(y), ptr(counter), ptr(used), seed & _M64, site, hi, lo, scale, x.numel())

@@ -9,8 +9,10 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from test_sequence_ops import INF, check_logprob, on_devices, on_types, rand  # noqa: E402
 
+from pytorch_distributed_amd.ops._seq import native  # noqa: E402
+from pytorch_distributed_amd.ops.dropout import dropout  # noqa: E402
 from pytorch_distributed_amd.ops.logprob import token_logprobs  # noqa: E402
-from pytorch_distributed_amd.ops.scan import linear_scan_step  # noqa: E402
+from pytorch_distributed_amd.ops.scan import linear_scan, linear_scan_step  # noqa: E402
 
 
 # ---- token log-probabilities ---------------------------------------------------------------------------------------
@@ -72,3 +74,52 @@ def test_a_state_that_a_graph_saved_is_not_overwritten_unseen(dev, second_buffer
         a = state.clone()
         b = linear_scan_step(x, g, a)
         assert torch.equal(a, b)
+
+
+# ---- together ------------------------------------------------------------------------------------------------------
+def calls(dev):
+    """-> {name: function of a [4, 60] tensor}"""
+    tok, ctr = torch.zeros(4, dtype=torch.int64, device=dev), torch.zeros(1, dtype=torch.int64, device=dev)
+    gate, state = torch.full((4, 60), 0.5, device=dev), rand((4, 60), torch.float32, dev, 2)
+    return {"logprob": lambda t: token_logprobs(t, tok).logprob, "scan": lambda t: linear_scan(t, gate)[0],
+            "step": lambda t: linear_scan_step(t, gate, state.clone()), "dropout": lambda t: dropout(t, 0.5, 1, ctr)}
+
+
+@on_devices
+@pytest.mark.parametrize("name", ["logprob", "scan", "step", "dropout"])
+@pytest.mark.parametrize("pre_dispatch", [False, True])
+def test_recorded_programs(dev, name, pre_dispatch):
+    """make_fx: on the CPU the formulas are recorded; a launch cannot be, and is refused."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, x, y = calls(dev)[name], rand((4, 60), torch.float32, dev, 0), rand((4, 60), torch.float32, dev, 1)
+    if dev == "cuda":
+        with pytest.raises(RuntimeError, match="traced program"):
+            make_fx(f, pre_dispatch=pre_dispatch)(x)
+        f(x)
+    else:
+        assert torch.equal(make_fx(f, pre_dispatch=pre_dispatch)(x)(y), f(y))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["logprob", "scan", "step", "dropout"])
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+def test_traces(name):
+    f, x = calls("cuda")[name], rand((4, 60), torch.float32, "cuda", 0)
+    with pytest.raises(RuntimeError, match="traced program"):
+        torch.jit.trace(f, (x,), check_trace=False)
+    if name == "dropout":       # with a gradient the call is one recorded operation
+        traced = torch.jit.trace(f, (x.clone().requires_grad_(),), check_trace=False)
+        y = rand((4, 60), torch.float32, "cuda", 1)
+        assert torch.equal(traced(y), f(y))
+
+
+def test_the_library_is_not_handed_to_a_tracer():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def f(t):
+        native("pda_scan_step")
+        return t
+    for how in (lambda: torch.jit.trace(f, (torch.zeros(2),), check_trace=False), lambda: make_fx(f)(torch.zeros(2)),
+                lambda: make_fx(f, pre_dispatch=True)(torch.zeros(2))):
+        with pytest.raises(RuntimeError, match="traced program"):
+            how()
