@@ -124,7 +124,11 @@ def dropout(x, p, seed, counter, site=0, residual=None):
 class CounterDropout(nn.Module):
     """Dropout layer on `dropout`: keeps its own step counter (a buffer that is no part of the state dict) and bumps it
     behind every call that dropped.  Active in training mode and where gradients are recorded, so action selection and
-    target values, which run under no_grad, never drop."""
+    target values, which run under no_grad, never drop.
+
+    Not for parts of a model that are computed again in the backward pass (activation checkpointing): the second computation
+    would read a counter that has gone on, so it is refused.  `dropout` with a counter of the caller's, bumped once per step
+    behind the backward pass, gives both computations the same mask."""
 
     def __init__(self, p, seed=0, site=0):
         super().__init__()
@@ -136,6 +140,9 @@ class CounterDropout(nn.Module):
     def forward(self, x, residual=None):
         if self.p == 0.0 or not self.training or not torch.is_grad_enabled():
             return x if residual is None else x + residual
+        if torch._C._current_graph_task_id() != -1:         # (inside a running backward pass)
+            raise RuntimeError("CounterDropout cannot be computed again in a backward pass (activation checkpointing): its "
+                               "counter has gone on; use ops.dropout.dropout with a counter bumped once per step")
         y = dropout(x, self.p, self.seed, self.counter, site=self.site, residual=residual)
         self.counter.add_(1)
         return y

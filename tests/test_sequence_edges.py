@@ -10,7 +10,7 @@ sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from test_sequence_ops import INF, check_logprob, on_devices, on_types, rand  # noqa: E402
 
 from pytorch_distributed_amd.ops._seq import native  # noqa: E402
-from pytorch_distributed_amd.ops.dropout import dropout  # noqa: E402
+from pytorch_distributed_amd.ops.dropout import CounterDropout, dropout  # noqa: E402
 from pytorch_distributed_amd.ops.logprob import token_logprobs  # noqa: E402
 from pytorch_distributed_amd.ops.scan import linear_scan, linear_scan_step  # noqa: E402
 
@@ -73,6 +73,30 @@ def test_a_state_that_a_graph_saved_is_not_overwritten_unseen(dev, second_buffer
     with torch.inference_mode():        # tensors without a version counter
         a = state.clone()
         b = linear_scan_step(x, g, a)
+        assert torch.equal(a, b)
+
+
+# ---- dropout -------------------------------------------------------------------------------------------------------
+@on_devices
+@pytest.mark.parametrize("use_reentrant", [False, True])
+def test_dropout_under_activation_checkpointing(dev, use_reentrant):
+    from torch.utils.checkpoint import checkpoint
+    x = rand((40, 25), torch.float32, dev, 1)
+    ctr = torch.full((1,), 6, dtype=torch.int64, device=dev)
+    drop = CounterDropout(0.5, seed=3).to(dev)
+
+    def gradient(f, again):
+        leaf = x.clone().requires_grad_()
+        y = checkpoint(f, leaf, use_reentrant=use_reentrant) if again else f(leaf)
+        y.sum().backward()
+        return y.detach(), leaf.grad
+    for a, b in zip(*(gradient(lambda t: dropout(t * 2, 0.5, 3, ctr).square(), again) for again in (False, True))):
+        assert torch.equal(a, b)
+    gradient(drop, False)
+    with pytest.raises(RuntimeError, match="checkpointing"):
+        gradient(lambda t: drop(t * 2).square(), True)
+    drop.eval()                         # nothing is dropped, nothing to disagree
+    for a, b in zip(*(gradient(lambda t: drop(t * 2).square(), again) for again in (False, True))):
         assert torch.equal(a, b)
 
 
