@@ -71,6 +71,14 @@ def wants_graph(*tensors):
     return getattr(forward_ad, "_current_level", -1) >= 0
 
 
+def refuse_tangents(name, *tensors):
+    """For operators without an autograd function, which would drop them."""
+    if getattr(forward_ad, "_current_level", -1) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("%s carries no tangents forward" % name)
+
+
 def ptr(t):
     return t.data_ptr() if t is not None else None
 

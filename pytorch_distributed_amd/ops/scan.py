@@ -11,7 +11,8 @@ import functools
 import torch
 from torch.autograd.graph import increment_version
 
-from ._seq import TYPE_CODES, check_floating, check_int, differentiable_once, launched, native, ptr, run_on, wants_graph
+from ._seq import TYPE_CODES, check_floating, check_int, differentiable_once, launched, native, ptr, refuse_tangents, run_on, \
+    wants_graph
 
 GATES = ("decay", "logit")
 _vp, _i64, _int = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
@@ -238,7 +239,8 @@ def linear_scan_step(x, gate, state, gates="decay", mix=False, state_out=None):
     to `state` itself, or to state_out, a second buffer (memory that overlaps state, x or gate otherwise than as the same view is refused).
 
     x, gate [B, D] of one type, state float32 [B, D]; any strides, but no element of the written buffer may be shared
-    (an expanded view is refused).  No gradient."""
+    (an expanded view is refused).  No gradient: h and the written state are no part of a graph, whatever x, gate and state
+    are; tangents carried forward are refused."""
     check_floating(x, "x")
     logit = _check_gates(gates)
     if x.dim() != 2:
@@ -250,6 +252,7 @@ def linear_scan_step(x, gate, state, gates="decay", mix=False, state_out=None):
     for t, what in ((gate, "gate"), (state, "state"), (out, "state_out")):
         if t.shape != x.shape:
             raise ValueError("%s has shape %s, x %s" % (what, tuple(t.shape), tuple(x.shape)))
+    refuse_tangents("linear_scan_step", x, gate, state, state_out)
     B, D = x.shape
     if not out.is_contiguous():
         (s0, n0), (s1, n1) = sorted(zip(out.stride(), out.shape))

@@ -76,6 +76,20 @@ def test_a_state_that_a_graph_saved_is_not_overwritten_unseen(dev, second_buffer
         assert torch.equal(a, b)
 
 
+@on_devices
+def test_the_step_refuses_tangents(dev):
+    from torch.autograd import forward_ad
+    x, g, state = (rand((3, 8), torch.float32, dev, i) for i in range(3))
+    want = linear_scan_step(x, g, state.clone())
+    with forward_ad.dual_level():
+        for i in range(4):
+            args = [x, g, state.clone(), torch.zeros_like(state)]
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(x))
+            with pytest.raises(NotImplementedError):
+                linear_scan_step(*args[:3], state_out=args[3])
+        assert torch.equal(linear_scan_step(x, g, state), want)
+
+
 # ---- dropout -------------------------------------------------------------------------------------------------------
 @on_devices
 @pytest.mark.parametrize("use_reentrant", [False, True])
