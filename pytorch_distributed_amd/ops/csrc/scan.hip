@@ -24,7 +24,8 @@ struct ScanArgs {
     int chunks, chunk_len, carry_len, carries;      // ScanPlan
 };
 
-// k = a where a <= 1/2, else -c (its sign says which); c = 1 - a.  For decay gates k = a.
+// k = a where a <= 1/2, else -c (its sign bit says which, also that of -0: a step that does not exist, and a gate saturated at
+// 1, have c = 0); c = 1 - a.  For decay gates k = a.
 struct Gate { float k, c; };
 template <bool LOGIT>
 __device__ __forceinline__ Gate gate_of(float g) {

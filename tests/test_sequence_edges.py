@@ -9,6 +9,7 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from test_sequence_ops import INF, check_logprob, on_devices, on_types, rand  # noqa: E402
 
+from pytorch_distributed_amd.ops import build  # noqa: E402
 from pytorch_distributed_amd.ops._seq import native  # noqa: E402
 from pytorch_distributed_amd.ops.dropout import CounterDropout, dropout  # noqa: E402
 from pytorch_distributed_amd.ops.logprob import token_logprobs  # noqa: E402
@@ -88,6 +89,31 @@ def test_the_step_refuses_tangents(dev):
             with pytest.raises(NotImplementedError):
                 linear_scan_step(*args[:3], state_out=args[3])
         assert torch.equal(linear_scan_step(x, g, state), want)
+
+
+def test_the_recurrence_is_built_with_signed_zeros():
+    """A gate that is saturated at 1, or whose step does not exist, is -0 in the kernels; without the sign the state is lost."""
+    flags = build.FLAGS + build.SOURCE_FLAGS["scan.hip"]
+    assert "-fsigned-zeros" in flags[flags.index("-ffast-math"):]
+
+
+@on_devices
+@on_types
+@pytest.mark.parametrize("d", [1, 40])
+def test_saturated_gates_keep_the_state(dev, dt, d):
+    x = torch.zeros(2, 70, d, dtype=dt, device=dev)
+    h0 = rand((2, d), torch.float32, dev, 1)
+    n = torch.tensor([70, 3], device=dev)
+    for logit in (200.0, INF):
+        gate = torch.full_like(x, logit).requires_grad_()
+        for mix in (False, True):
+            h, last = linear_scan(x, gate, h0, gates="logit", mix=mix, lengths=n)
+            assert torch.equal(last, h0) and torch.equal(h[0], h0[0].to(dt).expand(70, d)) and (h[1, 3:] == 0).all()
+            grad, = torch.autograd.grad(h.sum() + last.sum(), gate)
+            assert torch.equal(grad, torch.zeros_like(grad))
+            state = h0.clone()
+            assert torch.equal(linear_scan_step(x[:, 0], gate[:, 0].detach(), state, gates="logit", mix=mix), h0.to(dt))
+            assert torch.equal(state, h0)
 
 
 # ---- dropout -------------------------------------------------------------------------------------------------------
