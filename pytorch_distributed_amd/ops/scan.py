@@ -200,7 +200,9 @@ def linear_scan(x, gate, h0=None, gates="decay", mix=False, reverse=False, lengt
     h has x's shape and type and is contiguous; last is the float32 state behind the last step (h0 where a length is 0).
     The state is 32 bits wide throughout.  Gradients flow from h and last to x, gate and h0 (not twice).  Decay gates are
     meant to be within [-1, 1]; with larger ones, products of gates over a few hundred steps can overflow 32 bits and the
-    result is then inf or NaN even where the exact one is finite."""
+    result is then inf or NaN even where the exact one is finite.  A state that became infinite or NaN stays one of the two,
+    not always the one that the formula gives, in its own channel and from its own step on (of a sequence whose state is
+    infinite, last too)."""
     check_floating(x, "x")
     logit = _check_gates(gates)
     if x.dim() not in (2, 3):

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_sequence_ops import INF, check_logprob, on_devices, on_types, rand  # noqa: E402
+from test_sequence_ops import FORMS, INF, check_logprob, on_devices, on_types, rand, scan_inputs  # noqa: E402
 
 from pytorch_distributed_amd.ops import build  # noqa: E402
 from pytorch_distributed_amd.ops._seq import native  # noqa: E402
@@ -114,6 +114,22 @@ def test_saturated_gates_keep_the_state(dev, dt, d):
             state = h0.clone()
             assert torch.equal(linear_scan_step(x[:, 0], gate[:, 0].detach(), state, gates="logit", mix=mix), h0.to(dt))
             assert torch.equal(state, h0)
+
+
+@on_devices
+@pytest.mark.parametrize("gates,mix,reverse", FORMS)
+@pytest.mark.parametrize("t,d", [(60, 3), (700, 1), (900, 40)])
+def test_an_infinite_state_stays_in_its_channel(dev, gates, mix, reverse, t, d):
+    x, g = scan_inputs((2, t, d), torch.float32, dev, gates, seed=t)
+    n = torch.tensor([t, t - 20], device=dev)
+    clean, last = linear_scan(x, g, gates=gates, mix=mix, reverse=reverse, lengths=n)
+    y, at, c = x.clone(), t // 2, d - 1
+    y[1, at, c] = INF
+    h, fin = linear_scan(y, g, gates=gates, mix=mix, reverse=reverse, lengths=n)
+    behind = slice(0, at + 1) if reverse else slice(at, t - 20)
+    assert not torch.isfinite(h[1, behind, c]).any() and not torch.isfinite(fin[1, c])
+    h[1, behind, c], fin[1, c] = clean[1, behind, c], last[1, c]
+    assert torch.equal(h, clean) and torch.equal(fin, last)
 
 
 # ---- dropout -------------------------------------------------------------------------------------------------------
