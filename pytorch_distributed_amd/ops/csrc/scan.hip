@@ -88,8 +88,9 @@ template <typename T> struct ScanBwd {
     static constexpr int VEC = 16 / sizeof(T), CL = SCAN_CL, L = 32 / VEC, NT = 256;
 };
 // Fewer than 8 channels: one sequence of one channel per workgroup, of 16 waves or of one.  Latency is all that counts
-// there, so states and products are 64 bits wide: a constant gate such as 0.99 rounds every product the same way, which
-// left 5e-7 of 12500 discounted returns in 32 bits.
+// there, so a workgroup's states and products are 64 bits wide: a constant gate such as 0.99 rounds every product the same
+// way, which left 5e-7 of 12500 discounted returns in 32 bits.  What passes through memory is rounded to 32: the sums of
+// chunks, once for every 8192 steps or more, and the state that the backward pass starts a tile from.
 // (16 x 12500 fp32 returns: 8.7 us, of which the loads of the two tiles that a workgroup walks are most.)
 struct ScanRow { typedef double Acc; typedef ScanRow Sum; static constexpr int VEC = 1, CL = 1, L = 8, NT = 1024; };
 struct ScanWave { typedef double Acc; typedef void Sum; static constexpr int VEC = 1, CL = 1, L = 8, NT = 64; };

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_sequence_ops import FORMS, INF, check_logprob, on_devices, on_types, rand, scan_inputs  # noqa: E402
+from test_sequence_ops import FORMS, INF, check_logprob, check_scan, on_devices, on_types, rand, scan_inputs  # noqa: E402
 
 from pytorch_distributed_amd.ops import build  # noqa: E402
 from pytorch_distributed_amd.ops._seq import native  # noqa: E402
@@ -56,6 +56,17 @@ def test_logprob_masks_by_a_low_value_are_masks(dev, dt, v):
     for fill in (torch.finfo(dt).min, -3e4) + (() if dt == torch.float16 else (-1e9, -1e20)):
         for a, b in zip(run(fill), want):
             assert torch.equal(a, b), fill
+
+
+@pytest.mark.gpu
+@on_types
+@pytest.mark.parametrize("v", [1500, 9001])
+def test_logprob_gradient_rows_off_the_store_grid(dt, v):
+    """Logits and gradient rows of which most are not on the 16-byte grid together."""
+    big = rand((4, v + 9), dt, "cuda", 3, 2.0)
+    tokens = torch.tensor([0, 2, v // 2, v - 1], device="cuda")
+    for off in (1, 3):
+        check_logprob(big[:, off:off + v], tokens, T=0.9)
 
 
 # ---- linear recurrence ---------------------------------------------------------------------------------------------
@@ -130,6 +141,48 @@ def test_an_infinite_state_stays_in_its_channel(dev, gates, mix, reverse, t, d):
     assert not torch.isfinite(h[1, behind, c]).any() and not torch.isfinite(fin[1, c])
     h[1, behind, c], fin[1, c] = clean[1, behind, c], last[1, c]
     assert torch.equal(h, clean) and torch.equal(fin, last)
+
+
+def returns_like(shape, dev, seed):
+    x = rand(shape, torch.float32, "cpu", seed)
+    g = torch.full(shape, 0.995)
+    g[torch.rand(shape, generator=torch.Generator().manual_seed(seed + 1)) < 1e-3] = 0.0
+    return x.to(dev), g.to(dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,t,d", [(1, 57345, 1), (2, 70001, 1), (1, 57400, 3)])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("layout", ["contiguous", "strided"])
+def test_scan_one_channel_in_chunks(b, t, d, reverse, layout):
+    """Concatenated episodes: fewer than 8 channels and enough steps to be cut; lengths inside a chunk and at its end."""
+    x, g = returns_like((b, t, d), "cuda", t + d)
+    n = torch.tensor([t - 100, 16384][:b], device="cuda")
+    if layout == "strided":
+        x, g = (torch.stack([q, q, q], 3)[..., 1] for q in (x, g))
+    h0 = rand((b, d), torch.float32, "cuda", 7)
+    check_scan(x, g, h0, None if b == 1 else n, reverse=reverse)
+    if b == 1:
+        check_scan(x, g, None, n, reverse=reverse)
+
+
+@pytest.mark.gpu
+@on_types
+def test_scan_one_channel_in_chunks_types(dt):
+    x, g = scan_inputs((1, 57345, 1), dt, "cuda", "logit", seed=3)
+    check_scan(x, g, rand((1, 1), torch.float32, "cuda", 7), None, "logit", True, True)
+
+
+@pytest.mark.gpu
+@on_types
+@pytest.mark.parametrize("gates,mix,reverse", FORMS[1:3])
+def test_scan_many_chunks(dt, gates, mix, reverse):
+    """More chunks than a workgroup folds at a time, in either direction."""
+    t = 40001 if dt == torch.float32 else 20001
+    x, g = scan_inputs((1, t, 24), dt, "cuda", gates, seed=t)
+    h0 = rand((1, 24), torch.float32, "cuda", 7)
+    check_scan(x, g, h0, None, gates, mix, reverse)
+    check_scan(x, g, h0, torch.tensor([t - 1111], device="cuda"), gates, mix, reverse)
 
 
 # ---- dropout -------------------------------------------------------------------------------------------------------
