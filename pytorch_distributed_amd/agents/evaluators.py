@@ -49,15 +49,21 @@ def run_episodes(env, model, nepisodes, early_stop, device=torch.device("cpu"), 
 @torch.no_grad()
 def returns_report(trace, gamma, device=torch.device("cpu")):
     """-> (mean discounted return of the trace's episodes, mean over its steps of the model's value minus the return that
-    followed): G_t = r_t + gamma G_{t+1}, restarted behind every episode, as ONE reversed linear recurrence over all steps.
-    An episode that was cut short counts as ended there."""
+    followed): G_t = r_t + gamma G_{t+1} as ONE reversed linear recurrence, an episode per row (so that the CPU path, which goes
+    step by step, takes the longest episode's steps and not all of them).  An episode that was cut short counts as ended there."""
     if not trace:
         return 0.0, 0.0
-    rows = torch.tensor([(r, 0.0 if end else float(gamma), v) for r, end, v in trace], dtype=torch.float32).to(device)
-    returns, _ = linear_scan(rows[None, :, 0], rows[None, :, 1], reverse=True)
-    ends = [i for i, (_, end, _) in enumerate(trace) if end]
-    starts = [0] + [i + 1 for i in ends if i + 1 < len(trace)]
-    return float(returns[0, starts].mean()), float((rows[:, 2] - returns[0]).mean())
+    ends = [i + 1 for i, (_, end, _) in enumerate(trace) if end]
+    if not ends or ends[-1] != len(trace):
+        ends.append(len(trace))
+    n = torch.tensor([end - start for start, end in zip([0] + ends, ends)])
+    live = torch.arange(int(n.max()))[None, :] < n[:, None]
+    rewards = torch.zeros(live.shape)
+    rewards[live] = torch.tensor([r for r, _, _ in trace], dtype=torch.float32)
+    rewards, n, live = rewards.to(device), n.to(device), live.to(device)
+    returns, _ = linear_scan(rewards, torch.full_like(rewards, float(gamma)), reverse=True, lengths=n)
+    values = torch.tensor([v for _, _, v in trace], dtype=torch.float32).to(device)
+    return float(returns[:, 0].mean()), float((values - returns[live]).mean())
 
 
 def evaluator(process_ind, args, global_logs, evaluator_logs, env_prototype, model_prototype, global_model):

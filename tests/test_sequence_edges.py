@@ -256,3 +256,31 @@ def test_the_library_is_not_handed_to_a_tracer():
                 lambda: make_fx(f, pre_dispatch=True)(torch.zeros(2))):
         with pytest.raises(RuntimeError, match="traced program"):
             how()
+
+
+# ---- the evaluator's returns ---------------------------------------------------------------------------------------
+def test_returns_take_the_steps_of_the_longest_episode(monkeypatch):
+    from pytorch_distributed_amd.agents import evaluators
+    seen = []
+
+    def scan(x, *args, **kw):
+        seen.append(x.shape[1])
+        return linear_scan(x, *args, **kw)
+    monkeypatch.setattr(evaluators, "linear_scan", scan)
+    lengths = [3, 1, 40, 7, 12]
+    trace = [(float(i % 5) - 1.0, i + 1 == n, 0.25 * i) for n in lengths for i in range(n)]
+    for cut in (0, 2):                  # the last episode ended, or cut short
+        steps = trace[:len(trace) - cut]
+        want, bias, at = [], [], 0
+        for n in lengths[:-1] + [lengths[-1] - cut]:
+            g = 0.0
+            for r, _, v in reversed(steps[at:at + n]):
+                g = r + 0.9 * g
+                bias.append(v - g)
+            want.append(g)
+            at += n
+        ret, off = evaluators.returns_report(steps, 0.9)
+        # returns below 30, a memory of 10 steps, means of 61 values: 64 half steps of 30
+        assert abs(ret - sum(want) / len(want)) < 64 * 30 * 2.0 ** -24
+        assert abs(off - sum(bias) / len(bias)) < 64 * 30 * 2.0 ** -24
+    assert seen == [40, 40]
