@@ -57,22 +57,25 @@ def _steps(T, n, reverse, dev):
         yield pos, (i < n)[:, None]
 
 
-def _forward_torch(x, gate, h0, n, logit, mix, reverse):
+def _forward_torch(x, gate, h0, n, logit, mix, reverse, hist=None):
+    """-> (h, last); hist: a list that receives the state in front of every step"""
     B, T, D = x.shape
     row = torch.arange(B)
     h = h0.clone() if h0 is not None else torch.zeros(B, D)
-    out, hist = torch.zeros(B, T, D, dtype=x.dtype), []
+    out = torch.zeros(B, T, D, dtype=x.dtype)
     for pos, on in _steps(T, n, reverse, x.device):
-        hist.append(h)
+        if hist is not None:
+            hist.append(h)
         h = torch.where(on, _advance(h, x[row, pos], gate[row, pos], logit, mix), h)
         out[row, pos] = torch.where(on, h.to(x.dtype), out[row, pos])
-    return out, h, hist
+    return out, h
 
 
 def _backward_torch(x, gate, h0, n, logit, mix, reverse, dh, dlast):
     B, T, D = x.shape
     row = torch.arange(B)
-    hist = _forward_torch(x, gate, h0, n, logit, mix, reverse)[2]
+    hist = []
+    _forward_torch(x, gate, h0, n, logit, mix, reverse, hist)
     dx, dg = torch.zeros(B, T, D, dtype=x.dtype), torch.zeros(B, T, D, dtype=x.dtype)
     carry = dlast.clone() if dlast is not None else torch.zeros(B, D)
     for prev, (pos, on) in reversed(list(zip(hist, _steps(T, n, reverse, x.device)))):
@@ -115,9 +118,8 @@ def _forward(x, gate, h0, lengths, how, keep):
     (B, T, D), xs, wide = _sizes(x)
     if x.device.type == "cpu":
         if wide:
-            h, last, _ = _forward_torch(x, gate, h0, _lengths(lengths, B, T), *how)
-            return h, last, None
-        h, last, _ = _forward_torch(_cube(x), _cube(gate), _cube(h0), _lengths(lengths, B, T), *how)
+            return (*_forward_torch(x, gate, h0, _lengths(lengths, B, T), *how), None)
+        h, last = _forward_torch(_cube(x), _cube(gate), _cube(h0), _lengths(lengths, B, T), *how)
         return h.squeeze(2), last.squeeze(1), None
     entry = native("pda_scan_fwd")
     kw = {"dtype": torch.float32, "device": x.device}

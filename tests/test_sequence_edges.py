@@ -2,6 +2,7 @@
 ops/scan.py, ops/dropout.py), and calls that have to be refused."""
 import os
 import sys
+import weakref
 
 import pytest
 import torch
@@ -9,7 +10,7 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from test_sequence_ops import FORMS, INF, check_logprob, check_scan, on_devices, on_types, rand, scan_inputs  # noqa: E402
 
-from pytorch_distributed_amd.ops import build  # noqa: E402
+from pytorch_distributed_amd.ops import build, scan  # noqa: E402
 from pytorch_distributed_amd.ops._seq import native  # noqa: E402
 from pytorch_distributed_amd.ops.dropout import CounterDropout, dropout  # noqa: E402
 from pytorch_distributed_amd.ops.logprob import token_logprobs  # noqa: E402
@@ -185,6 +186,21 @@ def test_scan_many_chunks(dt, gates, mix, reverse):
     check_scan(x, g, h0, torch.tensor([t - 1111], device="cuda"), gates, mix, reverse)
 
 
+def test_the_cpu_path_keeps_no_states_that_nothing_reads(monkeypatch):
+    states, alive = [], []
+    advance = scan._advance
+
+    def watched(h, *args):
+        states.append(weakref.ref(h))
+        alive.append(sum(r() is not None for r in states))
+        return advance(h, *args)
+    monkeypatch.setattr(scan, "_advance", watched)
+    x = rand((2, 50, 8), torch.float32, "cpu", 1)
+    linear_scan(x, torch.full_like(x, 0.5))
+    linear_scan(x[..., 0].clone().requires_grad_(), torch.full_like(x[..., 0], 0.5))
+    assert len(alive) == 100 and max(alive) <= 2
+
+
 # ---- dropout -------------------------------------------------------------------------------------------------------
 @on_devices
 @pytest.mark.parametrize("use_reentrant", [False, True])
@@ -263,10 +279,10 @@ def test_returns_take_the_steps_of_the_longest_episode(monkeypatch):
     from pytorch_distributed_amd.agents import evaluators
     seen = []
 
-    def scan(x, *args, **kw):
+    def seen_scan(x, *args, **kw):
         seen.append(x.shape[1])
         return linear_scan(x, *args, **kw)
-    monkeypatch.setattr(evaluators, "linear_scan", scan)
+    monkeypatch.setattr(evaluators, "linear_scan", seen_scan)
     lengths = [3, 1, 40, 7, 12]
     trace = [(float(i % 5) - 1.0, i + 1 == n, 0.25 * i) for n in lengths for i in range(n)]
     for cut in (0, 2):                  # the last episode ended, or cut short
