@@ -28,28 +28,27 @@ def check_int(t, what, shape, device):
 
 _is_tracing, _dispatch_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
 _in_dispatch, _PRE_DISPATCH = torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
+_ENTRIES = {}
 
 
-def _recorded():
-    """Whether a tracer records the operations of this thread into a program (torch.jit.trace, make_fx)."""
-    if _is_tracing():
-        return True
-    if _dispatch_modes() or _in_dispatch(_PRE_DISPATCH):
-        from torch.fx.experimental.proxy_tensor import get_proxy_mode
-        return get_proxy_mode() is not None
-    return False
+def _proxied():
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    return get_proxy_mode() is not None
 
 
 def native(name, whole=False):
     """The C entry `name`; raises when the library is not there (a GPU tensor never falls back to eager torch), and where a
-    tracer records the call: a launch is no torch operation, so the program would hold the outputs' allocation and no launch.
-    whole: an autograd function runs the call, which torch.jit.trace records as one operation."""
-    if _recorded() and not (whole and _is_tracing()):
+    tracer (torch.jit.trace, make_fx) records the call: a launch is no torch operation, so the program would hold the outputs'
+    allocation and no launch.  whole: an autograd function runs the call, which torch.jit.trace records as one operation."""
+    if (_is_tracing() and not whole) or ((_dispatch_modes() or _in_dispatch(_PRE_DISPATCH)) and _proxied()):
         raise RuntimeError("%s on a GPU cannot be recorded into a traced program" % name)
-    try:
-        return getattr(lib(), name)
-    except RuntimeError:
-        raise RuntimeError("%s on a GPU needs the HIP library: %s" % (name, native_error()))
+    entry = _ENTRIES.get(name)
+    if entry is None:
+        try:
+            entry = _ENTRIES[name] = getattr(lib(), name)
+        except RuntimeError:
+            raise RuntimeError("%s on a GPU needs the HIP library: %s" % (name, native_error()))
+    return entry
 
 
 def differentiable_once(backward):
