@@ -364,12 +364,14 @@ struct LpList {
 // Each thread keeps running statistics, shifted once per 32 or 16 values.  The alternatives: each wave keeps its best keys
 // sorted over its lanes.  A value is looked at again only if it passes the wave's k-th best, which the first batch sets to
 // the k-th largest of the lanes' maxima; a wave of n values then inserts about k (2 + ln(n / 2048)) of them, each by a
-// ballot and a shift by one lane.  FILL: the first batch, which is all that a wave of a split row mostly sees, is ordered
+// ballot and a shift by one lane.  That is for rows in no particular order; of values in ascending order every one is inserted
+// (1024 x 32000 bf16, 8 alternatives: 34 us in random order, 622 ascending; 1 x 131072, 20: 10 + 5 and 27 + 15).  FILL: the first batch, which is all that a wave of a split row mostly sees, is ordered
 // at once instead (1 row of 131072 bf16, 20 alternatives: 11.4 -> 10.0 us; in the loop over a whole row the same code costs
 // more than it saves: 4096 rows 248 -> 277 us).
 //
 // 4096 x 32000 bf16 without alternatives, a tenth of the rows ignored: 48.5 us for 236 MB, 4.9 TB/s (a sum of 256 MB: 5.7).
-// 4096 x 131072 bf16 with 8 alternatives: 248 us, 4.3 TB/s (a sum of 1 GB reads 4.0).  Split rows are bound by the
+// 4096 x 131072 bf16 with 8 alternatives: 247 us, 4.3 TB/s, in one process, 261 to 280 in others of the same build (a sum of 1
+// GB reads 4.0 TB/s).  Half of every row masked with the type's lowest value: 4096 x 32000 45 us, as without.  Split rows are bound by the
 // latency of the chain of loads, joins and the second launch: 1 x 131072 10.0 + 4.6 us.  (Workgroups of 1024 threads with a
 // shared limit, so that fewer parts are joined: 16 to 32 us.)
 template <typename T, bool TOP, bool FILL>

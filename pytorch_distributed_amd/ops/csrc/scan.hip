@@ -68,8 +68,9 @@ __device__ __forceinline__ int scan_length(const ScanArgs& p, int b) {
 // Measured at 8 x 2048 x 2048 bf16, sigmoid gates, leaky average, lengths of 1024 to 2048 (256 workgroups, one per CU):
 // forward 53 us for 168 MB (3.2 TB/s), backward 98 us for 285 MB (2.9 TB/s).  Loads, arithmetic and stores of a tile follow
 // one another on a CU that holds one workgroup (backward: one wave per SIMD, which issues about 2500 vector instructions a
-// tile, 10000 of the tile's 15000 cycles), and the longest sequence sets the time.  At 1 x 65521 x 512 fp32 (16 slabs, 256 workgroups): 54 + 78 us forward for 268 +
-// 403 MB, 47 + 140 us backward for 268 + 671 MB, 4.8 to 5.7 TB/s: bound by memory, a third of it the second reading.
+// tile, 10000 of the tile's 15000 cycles), and the longest sequence sets the time.  At 1 x 65521 x 512 fp32 (16 slabs, 256
+// workgroups): 56 + 75 us forward for 268 + 403 MB, 47 + 142 us backward for 268 + 671 MB, 4.7 to 5.7 TB/s: bound by memory, a
+// third of it the second reading.
 #define SCAN_CL 8
 // scan_sum_kernel, either direction: 128 / 256 / 512 threads take 65 + 62 / 54 + 47 / 60 + 50 us (forward + backward) at
 // 1 x 65521 x 512 fp32
@@ -91,7 +92,8 @@ template <typename T> struct ScanBwd {
 // there, so a workgroup's states and products are 64 bits wide: a constant gate such as 0.99 rounds every product the same
 // way, which left 5e-7 of 12500 discounted returns in 32 bits.  What passes through memory is rounded to 32: the sums of
 // chunks, once for every 8192 steps or more, and the state that the backward pass starts a tile from.
-// (16 x 12500 fp32 returns: 8.7 us, of which the loads of the two tiles that a workgroup walks are most.)
+// (16 x 12500 fp32 returns: 8.7 us, of which the loads of the two tiles that a workgroup walks are most; 8 forward + 21
+// backward with a gradient, 11 for 1 x 25000, 10 + 5 forward and 10 + 14 backward for 1 x 65536 in 8 chunks.)
 struct ScanRow { typedef double Acc; typedef ScanRow Sum; static constexpr int VEC = 1, CL = 1, L = 8, NT = 1024; };
 struct ScanWave { typedef double Acc; typedef void Sum; static constexpr int VEC = 1, CL = 1, L = 8, NT = 64; };
 // The lanes of a wave: SW consecutive ones hold consecutive runs of steps of one group of VEC channels, so that a scan
@@ -103,7 +105,10 @@ template <typename S> struct ScanLane {
 };
 
 // How a kernel touches memory: element by element (any strides), in 16-byte accesses (contiguous channels on the 16-byte
-// grid), or so with stores past the caches.
+// grid), or so with stores past the caches.  All of a call's tensors decide together: rows of 2047 bf16 channels, or one
+// stride-0 gradient (that of h.sum()), take the first way.  8 x 2048 x 2048 bf16, no lengths: 49 us forward and 102 backward,
+// with the gradient of h.sum() 248 backward, with 2047 channels 153 and 354; 8 x 2048 fp32 with 1024 / 1023 channels 41 + 78 /
+// 75 + 152.
 #define SCAN_ANY 0
 #define SCAN_WIDE 1
 #define SCAN_STREAM 2
@@ -620,9 +625,13 @@ __global__ __launch_bounds__(S::NT) void scan_sum_kernel(ScanArgs p) {
 // How a problem is cut (the forward and the backward pass of one call agree on it: a function of the sizes alone).
 //
 // Chunks: where the slabs are fewer than the 256 CUs and there are at least SCAN_CHUNK_TILES tiles, the steps are cut into
-// as many chunks as give every CU one workgroup; with fewer tiles the second reading and its launch take longer than the
-// tiles that they save.  (Chunks taken in turns that fit the memory-side cache, so that the second reading finds them
-// there: 323 us against 326 us at 1 x 65521 x 512 fp32 with gradient, not worth it.)
+// as many chunks as give every CU one workgroup.  Forward + backward with the cut against without, sigmoid gates, leaky
+// average: 8 tiles, 32 slabs (1 x 2048 x 2048 bf16) 19 + 25 us against 42 + 87; 8 tiles, 128 slabs 46 + 69 against 43 + 89;
+// 16 tiles, 16 slabs (1 x 8192 x 512 fp32) 22 + 29 against more than 77 + 160.  With fewer tiles what it gains depends on the
+// slabs: 4 tiles, 128 slabs (4 x 1024 x 2048 bf16) 29 + 40 against 25 + 47, 4 tiles, 16 slabs (1 x 2048 x 512 fp32) 18 + 26
+// against 28 + 56: the rule leaves both as they are.  From 129 to 255 slabs a cut would give some CUs two workgroups: not taken.  (Chunks
+// taken in turns that fit the memory-side cache, so that the second reading finds them there: 323 us against 326 us at
+// 1 x 65521 x 512 fp32 with gradient, not worth it.)
 #define SCAN_CHUNK_TILES 8
 #define SCAN_ROUND 256
 struct ScanPlan { int kind, slabs, chunks, chunk_len, carry_len, carries; };
@@ -728,7 +737,8 @@ static int scan_run(const ScanArgs* args, int dtype, bool backward, hipStream_t 
 PDA_EXPORT int pda_scan_fwd(const ScanArgs* args, int dtype, hipStream_t stream) { return scan_run(args, dtype, false, stream); }
 PDA_EXPORT int pda_scan_bwd(const ScanArgs* args, int dtype, hipStream_t stream) { return scan_run(args, dtype, true, stream); }
 
-// One step of every request, a thread per element.  Bound by the launch: 64 x 2048 bf16 (1.8 MB) 2.7 us.
+// One step of every request, a thread per element.  Bound by the launch: 64 x 2048 bf16 (1.8 MB) 2.7 us; 512 x 8192 (59 MB)
+// 12.9 us, 4.6 TB/s; 4096 x 8192 (470 MB) 111 us, 4.2 TB/s.
 struct ScanStepArgs {
     const void* x; const void* gate; const float* state; float* state_out; void* h;
     long long xs[2], gs[2], ss[2], os[2];       // element strides (request, channel)

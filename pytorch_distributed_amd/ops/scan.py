@@ -240,7 +240,8 @@ def _span(t):
 
 def linear_scan_step(x, gate, state, gates="decay", mix=False, state_out=None):
     """One step of `linear_scan` for every request of a batch: h = a state + u, returned in x's type and written in 32 bits
-    to `state` itself, or to state_out, a second buffer (memory that overlaps state, x or gate otherwise than as the same view is refused).
+    to `state` itself, or to state_out, a second buffer.  Memory that overlaps state, x or gate otherwise than as the same view
+    is refused, and so are views that interleave, such as pool[:, 0] and pool[:, 1].
 
     x, gate [B, D] of one type, state float32 [B, D]; any strides, but no element of the written buffer may be shared
     (an expanded view is refused).  No gradient: h and the written state are no part of a graph, whatever x, gate and state
