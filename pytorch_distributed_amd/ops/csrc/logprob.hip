@@ -59,10 +59,13 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 // d = x c - r
 struct LpStat { float m, s, u; };
 #define LP_LN2 0.693147180559945309f
-// The rounding of r is at most |r| 2^-24: below this bound 2^(its rounding) stays near 1.  Beyond it d = (x - m) c: in a part
-// that holds nothing but masks of a low value, and in rows whose maximum lies there (logits of more than 7e6 T, masks in
-// every place), which are walked once more because their parts' references cannot be told apart.
+// The rounding of r is at most |r| 2^-24: below LP_NEAR 2^(its rounding) stays near 1.  Rows whose maximum lies beyond it
+// (logits of more than 7e6 T, masks of the type's lowest value in every place) are walked once more with d = (x - m) c.
+// A part's s stays below 2^32 for each of its values up to LP_FAR, where r is rounded to multiples of 64.  A part beyond that,
+// nothing but masks of a low value, takes d = (x - m) c too: how it stands to another part's r is not known, and need not be,
+// because a row whose maximum is near drops it.
 #define LP_NEAR 1.0e7f
+#define LP_FAR 1.0e9f
 __device__ __forceinline__ float lp_exp2(float d) { return __builtin_amdgcn_exp2f(d); }
 __device__ __forceinline__ float lp_ref(float m, float c) {
     float r = m * c;
@@ -70,8 +73,8 @@ __device__ __forceinline__ float lp_ref(float m, float c) {
     return r;
 }
 __device__ __forceinline__ bool lp_near(float r) { return fabsf(r) < LP_NEAR; }
-// `st` seen from the maximum m >= st.m (no part of it turns into 0 * inf: the shift is cut off where 2^shift is 0, and s, a
-// count of at most the row's tokens up to r's rounding, is finite)
+// `st` seen from the maximum m >= st.m.  No part of it turns into 0 * inf, unless the row is walked: the shift is cut off where
+// 2^shift is 0, and s < 2^62 times a shift of 2e9, or a far part's s < 2^30 times the cut-off, is finite.
 __device__ __forceinline__ LpStat lp_shift(LpStat st, float m, float c) {
     const float d = st.m == m ? 0.f : fmaxf(lp_ref(st.m, c) - lp_ref(m, c), -1.0e20f), e = lp_exp2(d);
     return LpStat{m, st.s * e, e * __builtin_fmaf(d, st.s, st.u)};
@@ -88,14 +91,14 @@ __device__ __forceinline__ void lp_add(LpStat& st, const float (&x)[NX], float b
     st = lp_shift(st, fmaxf(st.m, bm), c);
     const float r = st.m == -INFINITY ? 0.f : lp_ref(st.m, c);
     float s = 0.f, u = 0.f;
-    if (lp_near(r)) {
+    if (fabsf(r) < LP_FAR) {
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
             const float d = __builtin_fmaf(x[i], c, -r), e = lp_exp2(d);
             s += e;                                             // (NaN for a NaN)
             u = __builtin_fmaf(e, fmaxf(d, -1000.f), u);        // (0 for -inf)
         }
-    } else {        // nothing but masks of a low value so far (or a row that will be walked): s stays finite, and a larger maximum drops it
+    } else {            // (NaN for +inf)
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
             const float d = (x[i] - st.m) * c, e = lp_exp2(d);

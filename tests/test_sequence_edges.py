@@ -4,11 +4,14 @@ import os
 import sys
 import weakref
 
+import numpy as np
 import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_sequence_ops import FORMS, INF, check_logprob, check_scan, on_devices, on_types, rand, scan_inputs  # noqa: E402
+import sequence_oracle as oracle  # noqa: E402
+from test_sequence_ops import FORMS, INF, check_logprob, check_scan, close, np64, on_devices, on_types, rand, rounding, \
+    scan_inputs  # noqa: E402
 
 from pytorch_distributed_amd.ops import build, scan  # noqa: E402
 from pytorch_distributed_amd.ops._seq import native  # noqa: E402
@@ -54,9 +57,33 @@ def test_logprob_masks_by_a_low_value_are_masks(dev, dt, v):
         d, = torch.autograd.grad(o.logprob.sum() + o.entropy.sum() + o.logsumexp.sum(), x)
         return [o.logprob, o.entropy, o.logsumexp, o.top_logprobs, o.top_tokens, d]
     want = run(-INF)
-    for fill in (torch.finfo(dt).min, -3e4) + (() if dt == torch.float16 else (-1e9, -1e20)):
+    for fill in (torch.finfo(dt).min, -3e4) + (() if dt == torch.float16 else (-5e8, -1e9, -1e20)):
         for a, b in zip(run(fill), want):
             assert torch.equal(a, b), fill
+
+
+@on_devices
+@pytest.mark.parametrize("v", [2500, 20000])
+@pytest.mark.parametrize("around", [-6931471.5, 6931472.0, -6.931472e8, -7.0e5])
+def test_logprob_rows_of_large_logits(dev, v, around):
+    """Logits whose exponents' references lie on either side of the bounds at which a part or a row changes its form."""
+    x = rand((5, v), torch.float32, "cpu", v, 1.0) * torch.tensor([[2.0], [20.0], [200.0], [2000.0], [0.0]]) + around
+    x[4, :v // 2] -= 0.5                # whole parts on one side, the row's maximum on the other
+    x = x.to(dev)
+    tokens = torch.tensor([0, 7, v // 2, v - 1, 0], device=dev)
+    leaf = x.clone().requires_grad_()
+    out = token_logprobs(leaf, tokens, top_k=3)
+    up = [rand((5,), torch.float32, dev, i) for i in range(3)]
+    d, = torch.autograd.grad(out[:3], leaf, up)
+    want, tol, dx, dtol = oracle.logprob(np64(x), tokens.cpu().numpy(), 1.0, -100, *[np64(t) for t in up])
+    for name, got in (("lp", out.logprob), ("ent", out.entropy), ("lse", out.logsumexp)):
+        close(got, want[name], tol[name])
+    assert torch.equal(out.top_tokens.cpu(), torch.sort(x.cpu(), dim=1, descending=True, stable=True)[1][:, :3])
+    # a probability below 2^-126 may be taken as 0: p k with |k| <= |dlse| + |dlp| + |dent| (|logp| + entropy), and at that
+    # border |logp| is 88, while p falls faster than |logp| rises behind it
+    a, b, c = (np.abs(np64(t)) for t in up)
+    flushed = 2.0 ** -126 * (a + c + b * (88 + want["ent"]))
+    close(d, dx, dtol + flushed[:, None] + rounding(torch.float32, dx))
 
 
 @pytest.mark.gpu
