@@ -55,11 +55,9 @@ def _threshold(p):
 
 
 def _run(x, residual, p, seed, site, counter, used):
-    """y = x scaled where kept (+ residual); used: int64[1] that receives the counter's value (None: backward pass)."""
+    """y = x scaled where kept (+ residual); used: int64[1] that receives the counter's value on a GPU (None: backward pass)."""
     scale = 1.0 / (1.0 - p) if p < 1.0 else 0.0
     if x.device.type == "cpu":
-        if used is not None:
-            used.copy_(counter)
         keep = keep_mask(x.numel(), p, seed, counter, site).reshape(x.shape)
         y = torch.where(keep, x.float() * scale, torch.zeros(()))
         return (y if residual is None else y + residual.float()).to(x.dtype)
@@ -74,8 +72,13 @@ def _run(x, residual, p, seed, site, counter, used):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, site, counter):
-        used = torch.empty_like(counter)
-        y = _run(x.contiguous(), residual.contiguous() if residual is not None else None, p, seed, site, counter, used)
+        x, residual = x.contiguous(), residual.contiguous() if residual is not None else None
+        if x.device.type == "cpu":
+            used = counter.clone()
+            y = _run(x, residual, p, seed, site, used, None)
+        else:
+            used = torch.empty_like(counter)
+            y = _run(x, residual, p, seed, site, counter, used)
         ctx.save_for_backward(used)
         ctx.how = (p, seed, site)
         return y
@@ -128,7 +131,7 @@ class CounterDropout(nn.Module):
 
     Not for parts of a model that are computed again in the backward pass (activation checkpointing): the second computation
     would read a counter that has gone on, so it is refused.  `dropout` with a counter of the caller's, bumped once per step
-    behind the backward pass, gives both computations the same mask."""
+    behind the backward pass, gives both computations the same mask.  (For the same check torch.compile breaks its graph here.)"""
 
     def __init__(self, p, seed=0, site=0):
         super().__init__()

@@ -252,6 +252,23 @@ def test_dropout_under_activation_checkpointing(dev, use_reentrant):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_the_dropout_layer_in_a_compiled_function(backend):
+    from torch.utils.checkpoint import checkpoint
+    torch._dynamo.reset()
+    one, two = CounterDropout(0.5, seed=3), CounterDropout(0.5, seed=3)
+    x = rand((40, 25), torch.float32, "cpu", 1).requires_grad_()
+    f = torch.compile(lambda t: one(t * 2).square(), backend=backend)
+    for _ in range(2):
+        y, z = f(x), two(x * 2).square()
+        assert torch.equal(y, z) and int(one.counter) == int(two.counter)
+        for a, b in zip(torch.autograd.grad(y.sum(), x), torch.autograd.grad(z.sum(), x)):
+            assert torch.equal(a, b)
+    again = torch.compile(lambda t: checkpoint(lambda q: one(q * 2).square(), t, use_reentrant=False), backend=backend)
+    with pytest.raises(RuntimeError, match="checkpointing"):
+        torch.autograd.grad(again(x).sum(), x)
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 def calls(dev):
     """-> {name: function of a [4, 60] tensor}"""
